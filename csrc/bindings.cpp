@@ -82,6 +82,24 @@ void head_fwd_bwd(const torch::Tensor& y2, const c10::optional<torch::Tensor>& y
                   const c10::optional<torch::Tensor>& db, const c10::optional<torch::Tensor>& dgamma,
                   const c10::optional<torch::Tensor>& dbeta, const c10::optional<torch::Tensor>& dy2,
                   const c10::optional<torch::Tensor>& dy1);
+// embedding.cu
+void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tensor out, double scale);
+void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Tensor dw, double scale, int64_t padding_idx,
+                   bool accumulate);
+// qk_rope.cu
+void qk_norm_rope_fwd(const torch::Tensor& qkv, torch::Tensor out, int64_t heads, int64_t kv_heads,
+                      const c10::optional<torch::Tensor>& wq, const c10::optional<torch::Tensor>& wk, double eps,
+                      const c10::optional<torch::Tensor>& cos, const c10::optional<torch::Tensor>& sin,
+                      const c10::optional<torch::Tensor>& positions, const c10::optional<int64_t>& S, bool interleaved);
+void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch::Tensor dqkv, int64_t heads,
+                      int64_t kv_heads, const c10::optional<torch::Tensor>& wq, const c10::optional<torch::Tensor>& wk,
+                      const c10::optional<torch::Tensor>& dwq, const c10::optional<torch::Tensor>& dwk, double eps,
+                      const c10::optional<torch::Tensor>& cos, const c10::optional<torch::Tensor>& sin,
+                      const c10::optional<torch::Tensor>& positions, const c10::optional<int64_t>& S, bool interleaved,
+                      bool accumulate);
+// grad_clip.cu
+torch::Tensor clip_grads(const std::vector<torch::Tensor>& grads, double max_norm,
+                         const c10::optional<std::vector<torch::Tensor>>& out, bool max_type);
 // host.cpp
 void set_sm_reserve(int n);
 int sm_reserve();
@@ -142,6 +160,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("hb") = py::none(), py::arg("dpooled") = py::none(), py::arg("dW") = py::none(),
         py::arg("db") = py::none(), py::arg("dgamma") = py::none(), py::arg("dbeta") = py::none(),
         py::arg("dy2") = py::none(), py::arg("dy1") = py::none());
+  m.def("embedding_fwd", &revpp::embedding_fwd, py::arg("ids"), py::arg("w"), py::arg("out"), py::arg("scale"));
+  m.def("embedding_bwd", &revpp::embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("dw"), py::arg("scale"),
+        py::arg("padding_idx"), py::arg("accumulate"));
+  m.def("qk_norm_rope_fwd", &revpp::qk_norm_rope_fwd, py::arg("qkv"), py::arg("out"), py::arg("heads"),
+        py::arg("kv_heads"), py::arg("wq"), py::arg("wk"), py::arg("eps"), py::arg("cos"), py::arg("sin"),
+        py::arg("positions"), py::arg("S"), py::arg("interleaved"));
+  m.def("qk_norm_rope_bwd", &revpp::qk_norm_rope_bwd, py::arg("dout"), py::arg("qkv"), py::arg("dqkv"),
+        py::arg("heads"), py::arg("kv_heads"), py::arg("wq"), py::arg("wk"), py::arg("dwq"), py::arg("dwk"),
+        py::arg("eps"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("S"), py::arg("interleaved"),
+        py::arg("accumulate"));
+  m.def("clip_grads", &revpp::clip_grads, py::arg("grads"), py::arg("max_norm"), py::arg("out"), py::arg("max_type"));
   m.def("dp_reduce_adamw", &revpp::dp_reduce_adamw);
   m.def("pointer_info", &revpp::pointer_info);
   m.def("ipc_open", [](py::bytes h) { return revpp::ipc_open(std::string(h)); });

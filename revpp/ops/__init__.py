@@ -99,8 +99,94 @@ def attention_bwd(qkv, out, dout, lse, dqkv, dq_acc, dbuf, B, S, heads, colsum=N
             cast_colsum(dqkv, colsum=colsum)
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as [rows, last dimension] without a copy."""
+    return t if t.dim() == 2 else t.view(-1, t.shape[-1])
+
+
+def _ids(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def embedding_fwd(ids: torch.Tensor, w: torch.Tensor, out: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """out[..., :] = scale * w[ids[...]]   (token-embedding lookup).
+
+    ``ids`` int64 / int32 of any shape, ``w`` [V, H] and ``out`` [..., H] each fp32, bf16 or
+    fp16, contiguous along H (rows may lie further apart).  An id outside the table sets the
+    status word (``check_status``) and gives a row of zeros."""
+    ext().embedding_fwd(_ids(ids), w, _rows(out), scale)
+    return out
+
+
+def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dw: torch.Tensor, scale: float = 1.0,
+                  padding_idx: Optional[int] = None, accumulate: bool = True) -> torch.Tensor:
+    """dw[v] (+)= scale * sum of dy[t] over the tokens with ids[t] = v   (gradient of ``embedding_fwd``).
+
+    ``dy`` [..., H] fp32, bf16 or fp16, ``dw`` [V, H] fp32.  The tokens of ``padding_idx`` and ids
+    outside the table add nothing.  ``accumulate=False`` writes all of ``dw``, with zeros in the rows
+    that no token names.  The tokens are sorted first and each row is added in token order: equal
+    inputs give equal bits, unlike the atomics of ``bert_embed_bwd``."""
+    V = dw.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    elif not -V <= padding_idx < V:
+        raise ValueError(f"padding_idx {padding_idx} is outside the table's {V} rows")
+    elif padding_idx < 0:
+        padding_idx += V
+    ext().embedding_bwd(_rows(dy), _ids(ids), dw, scale, padding_idx, accumulate)
+    return dw
+
+
+def qk_norm_rope_fwd(qkv: torch.Tensor, out: torch.Tensor, heads: int, kv_heads: Optional[int] = None,
+                     wq: Optional[torch.Tensor] = None, wk: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                     cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                     positions: Optional[torch.Tensor] = None, S: Optional[int] = None,
+                     interleaved: bool = False) -> torch.Tensor:
+    """RMS norm of every query and key head, then the position rotation, on a packed projection.
+
+    ``qkv`` and ``out`` are [M, (heads + 2 * kv_heads) * d] (fp32, bf16 or fp16, d <= 256, rows may
+    lie further apart); ``kv_heads`` defaults to ``heads``, which is the layout that
+    ``attention_fwd`` reads.  ``out`` may be ``qkv`` itself; otherwise the value heads are copied.
+    ``wq`` / ``wk`` are the fp32 [d] norm weights (None: 1).  ``cos`` / ``sin`` (fp32 [P, rot / 2], None:
+    no rotation) turn the first ``rot`` columns of a head in pairs (i, i + rot / 2), or (2i, 2i + 1)
+    with ``interleaved``; row m takes the angles of ``positions[m]`` (int64 / int32 [M]), or of
+    ``m % S``.  A position outside the tables sets the status word and leaves its row unrotated."""
+    ext().qk_norm_rope_fwd(qkv, out, heads, heads if kv_heads is None else kv_heads, wq, wk, eps, cos, sin, positions,
+                           S, interleaved)
+    return out
+
+
+def qk_norm_rope_bwd(dout: torch.Tensor, qkv: torch.Tensor, dqkv: torch.Tensor, heads: int,
+                     kv_heads: Optional[int] = None, wq: Optional[torch.Tensor] = None,
+                     wk: Optional[torch.Tensor] = None, dwq: Optional[torch.Tensor] = None,
+                     dwk: Optional[torch.Tensor] = None, eps: float = 1e-6, cos: Optional[torch.Tensor] = None,
+                     sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                     S: Optional[int] = None, interleaved: bool = False, accumulate: bool = True) -> torch.Tensor:
+    """Gradient of ``qk_norm_rope_fwd``: ``dqkv`` from ``dout`` and the projection ``qkv`` as it was
+    before the norm.  ``dqkv`` may be ``dout`` itself (value heads stay), otherwise the value heads'
+    gradient is copied.  ``dwq`` / ``dwk`` (fp32 [d], optional) receive the norm weights' gradients:
+    added, or written with ``accumulate=False``; their sums are taken in a fixed order."""
+    ext().qk_norm_rope_bwd(dout, qkv, dqkv, heads, heads if kv_heads is None else kv_heads, wq, wk, dwq, dwk, eps, cos,
+                           sin, positions, S, interleaved, accumulate)
+    return dqkv
+
+
+def clip_grads(grads, max_norm: float, out=None, norm_type: float = 2.0) -> torch.Tensor:
+    """Scale many gradient tensors by min(1, max_norm / (norm + 1e-6)) and return their global norm
+    (fp32 scalar on the device, no synchronisation).
+
+    ``grads``: dense fp32 / bf16 / fp16 tensors on one device, of any number and sizes.  ``out``: where
+    the scaled gradients go (same sizes and strides, any of the three types), by default the gradients
+    themselves.  ``norm_type`` is 2 or inf.  Squares are summed in 64 bits in a fixed order.  A NaN in
+    any gradient makes the norm and every output NaN."""
+    if norm_type not in (2.0, float("inf")):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    return ext().clip_grads(grads, max_norm, out, norm_type != 2.0)
+
+
 __all__ = [
     "available", "check_status", "ext", "set_sm_reserve", "linear", "linear_dgrad", "linear_wgrad",
     "layernorm_fwd", "layernorm_bwd", "cast_colsum", "attention_fwd", "attention_bwd",
+    "embedding_fwd", "embedding_bwd", "qk_norm_rope_fwd", "qk_norm_rope_bwd", "clip_grads",
     "EPI_BF16", "EPI_GELU", "EPI_RESID", "EPI_ATOMIC", "EPI_DGELU", "EPI_F32",
 ]

@@ -12,7 +12,7 @@ shadow weights and zeroes the gradients.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Iterable, Optional, Sequence
 
 import torch
 import torch.distributed as dist
@@ -94,6 +94,42 @@ class StepLR:
         self.epoch += 1
         if self.epoch % self.step_size == 0:
             self.opt.lr *= self.gamma
+
+
+def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
+               norm_type: float = 2.0) -> torch.Tensor:
+    """Clip separate gradient tensors by their global norm, as ``FlatAdamW`` does for a flat buffer.
+
+    For parameters that live outside ``FlatParams`` (modules split by ``parallel.tracer``): scales every
+    gradient by min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (for instance the
+    ``FlatParams.grad_of`` views), and returns the norm (fp32 scalar).  CUDA tensors go through the
+    kernels (``ops.clip_grads``), CPU tensors through PyTorch."""
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(())
+    if grads[0].is_cuda:
+        from revpp import ops
+
+        return ops.clip_grads(grads, max_norm, out, norm_type)
+    if norm_type not in (2.0, float("inf")):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"out must have one tensor per gradient: {len(outs)} for {len(grads)}")
+    if any(o.shape != g.shape for o, g in zip(outs, grads)):
+        raise ValueError("out must have its gradients' sizes")
+    with torch.no_grad():
+        full = [g.double() for g in grads if g.numel()]
+        if norm_type == 2.0:
+            norm = sum((g.square().sum() for g in full), torch.zeros((), dtype=torch.float64)).sqrt()
+        else:
+            norm = torch.stack([g.abs().max() for g in full]).max() if full else torch.zeros((), dtype=torch.float64)
+        coef = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
+        for g, o in zip(grads, outs):
+            o.copy_(g.float() * coef)
+    return norm.float()
 
 
 def allreduce_sumsq(sumsq: torch.Tensor, group=None) -> torch.Tensor:
