@@ -10,16 +10,19 @@
 // arrive; here the tokens are sorted by id (stable, so each row's terms come in token order)
 // and every dW row is written once, so equal inputs give equal bits.
 //
-//  1. embed_sort_kernel: each CTA owns a range of ids, reads all n ids, counts those below
-//     its range (its offset in the sorted order, with no exchange between CTAs) and places its
-//     own by a counting sort.  Warp w reads the w-th part of the tokens and keeps its own
+//  1. embed_sort_kernel: 2^c CTAs, each owns the ids with its own low c bits (frequent tokens,
+//     which vocabularies number low, spread over the CTAs), reads all n ids, counts those of the
+//     CTAs before it (its offset in the sorted order, with no exchange between CTAs) and places
+//     its own by a counting sort.  Warp w reads the w-th part of the tokens and keeps its own
 //     counters, so that the order within an id is the token order.
-//  2. embed_reduce_kernel: one warp per (32 sorted tokens, slab of columns) adds the rows of
-//     each run of equal ids in registers.  A run inside the 32 goes straight to dW; a run
-//     that crosses into neighbouring chunks leaves its pieces in the workspace, and the warp
-//     that delivers the last piece adds them in chunk order (in groups of 32 for long runs).
-//     Without accumulation, further warps write zeros to the rows that no token names.
+//  2. embed_reduce_kernel: one CTA per (chunk of sorted tokens, slab of columns).  Each warp adds
+//     the rows of its part of the chunk run by run in registers and writes the runs that lie
+//     inside; runs that cross warps meet in shared memory, and runs that cross chunks leave one
+//     piece per chunk in the workspace.  Without accumulation, further CTAs write zeros to the rows
+//     that no token names.
+//  3. embed_join_kernel: adds the pieces of each run that crosses chunks, in chunk order.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "host.h"
@@ -32,9 +35,14 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kFwdUnroll = 4;      // vectors per lane and row slab
 constexpr int kSortWarps = 32;
-constexpr int kSortList = 256;     // matches a warp keeps between the two sweeps
-constexpr int kSortRange = 512;    // ids per CTA at most
-constexpr int kChunk = 32;         // sorted tokens per reduce task
+constexpr int kSortPer = 1024;     // tokens a warp lists at most before they are placed
+constexpr int kSortLogCtas = 7;    // at most one CTA per SM, unless the table is very long
+constexpr int kSortLogRange = 9;   // ids per CTA: 512 at most
+constexpr int kWarps = 4;          // of a reduce CTA
+constexpr int kWarpTokens = 8;    // sorted tokens a reduce warp adds: all their rows are in flight at once
+constexpr int kChunk = kWarps * kWarpTokens;
+constexpr int kLaneColumns = 8;    // columns of a reduce lane
+constexpr int kSlab = 32 * kLaneColumns;
 constexpr int kZeroRows = 8;       // dW rows per zero-writing warp
 
 // ------------------------------------------------------------------ forward
@@ -78,140 +86,204 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------ backward: sort
+// An id's place in the sorted order follows from its slot: the CTA that sorts it, then the rest.
 struct EmbedWs {
-  int* start;     // [vocab + 1] first sorted position of each id
+  int* start;     // [slots + 1] first sorted position of each slot
   int* order;     // [n] token of each sorted position
-  int* key;       // [n] id of each sorted position
-  int* count;     // [3][slabs][chunks] pieces delivered
-  float* part;    // [2][chunks][H] pieces of runs that cross chunks
+  int* key;       // [n] slot of each sorted position
+  float* part;    // [2][chunks][H] pieces of runs that cross chunks: from before, and into the next
+  int log_c, log_r;
+  __device__ __forceinline__ int slots() const { return 1 << (log_c + log_r); }
+  __device__ __forceinline__ int slot_of(int id) const { return ((id & ((1 << log_c) - 1)) << log_r) | (id >> log_c); }
+  __device__ __forceinline__ int id_of(int slot) const { return ((slot & ((1 << log_r) - 1)) << log_c) | (slot >> log_r); }
 };
 
-// The tokens of one warp whose id lies in [lo, lo + range), in token order, 32 at a time at
-// most: fn(token, local id, active).  Returns through `less` the number of ids below lo.
-template <typename TI, typename F>
-__device__ __forceinline__ void sweep(const TI* __restrict__ ids, int beg, int end, long long vocab, long long padding,
-                                      int lo, int range, int lane, int* list_tok, int* list_id, int& len, int& less,
-                                      bool& bad, bool& spilled, F&& fn) {
-  len = 0;
-  for (int t0 = beg; t0 < end; t0 += 8 * 32) {
-    int k[8];
+// The low 32 bits of an id inside the table, or ~0 for one outside.
+__device__ __forceinline__ unsigned checked(int64_t id, unsigned vocab) {
+  const unsigned lo = static_cast<unsigned>(id), hi = static_cast<unsigned>(static_cast<uint64_t>(id) >> 32);
+  return hi == 0 && lo < vocab ? lo : 0xffffffffu;
+}
+__device__ __forceinline__ unsigned checked(int32_t id, unsigned vocab) {
+  const unsigned lo = static_cast<unsigned>(id);
+  return lo < vocab ? lo : 0xffffffffu;
+}
+
+// The tokens [beg, end) of one warp whose slots belong to CTA `cta` go to `list` in token order, as
+// (token - seg) << 9 | local id, and are counted per local id; returns how many.  `less` counts the
+// ids of earlier CTAs.  A lane reads two neighbouring ids per access (`wide`: the address allows it).
+template <typename TI>
+__device__ __forceinline__ int sweep(const TI* __restrict__ ids, int seg, int beg, int end, bool wide, unsigned vocab,
+                                     unsigned padding, unsigned cta, int log_c, int lane, int* list, int* count, int& less,
+                                     bool& bad) {
+  constexpr int kPairs = 8;
+  const unsigned low = (1u << log_c) - 1, before = (1u << lane) - 1;
+  int len = 0;
+  for (int t0 = beg; t0 < end; t0 += kPairs * 64) {
+    unsigned id[kPairs][2];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int t = t0 + 32 * u + lane;
-      long long id = -1;
-      if (t < end) {
-        id = static_cast<long long>(ids[t]);
-        bad |= id < 0 || id >= vocab;
+    for (int u = 0; u < kPairs; ++u) {
+      const int t = t0 + 64 * u + 2 * lane;
+      if (wide && t0 + 64 * u + 64 <= end) {
+        using Raw = typename RawOf<2 * sizeof(TI)>::type;
+        const Raw raw = __ldg(reinterpret_cast<const Raw*>(ids + t));
+        id[u][0] = checked(reinterpret_cast<const TI*>(&raw)[0], vocab);
+        id[u][1] = checked(reinterpret_cast<const TI*>(&raw)[1], vocab);
+        if (cta == 0) bad |= id[u][0] == 0xffffffffu || id[u][1] == 0xffffffffu;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          id[u][e] = 0xffffffffu;
+          if (t + e < end) {
+            id[u][e] = checked(__ldg(ids + t + e), vocab);
+            bad |= id[u][e] == 0xffffffffu;
+          }
+        }
       }
-      k[u] = (id >= 0 && id < vocab && id != padding) ? static_cast<int>(id) : 0x7fffffff;
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      less += k[u] < lo;
-      const bool in = static_cast<unsigned>(k[u] - lo) < static_cast<unsigned>(range);
-      const unsigned m = __ballot_sync(0xffffffffu, in);
-      if (m == 0) continue;
-      if (len > kSortList - 32) {
-        spilled = true;
-        __syncwarp();
-        for (int i = 0; i < len; i += 32) fn(list_tok, list_id, i, len);
-        len = 0;
-        __syncwarp();
+    for (int u = 0; u < kPairs; ++u) {
+      if (t0 + 64 * u >= end) break;
+      bool in[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned k = id[u][e];
+        const unsigned c = k == padding || k == 0xffffffffu ? 0xffffffffu : k & low;
+        less += c < cta;
+        in[e] = c == cta;
       }
-      if (in) {
-        const int at = len + __popc(m & ((1u << lane) - 1));
-        list_tok[at] = t0 + 32 * u + lane;
-        list_id[at] = k[u] - lo;
-      }
-      len += __popc(m);
+      if (!__any_sync(0xffffffffu, in[0] || in[1])) continue;
+      const unsigned m0 = __ballot_sync(0xffffffffu, in[0]), m1 = __ballot_sync(0xffffffffu, in[1]);
+      int at = len + __popc(m0 & before) + __popc(m1 & before);
+      const int t = t0 - seg + 64 * u + 2 * lane;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (in[e]) {
+          const int local = static_cast<int>(id[u][e] >> log_c);
+          list[at++] = (t + e) << kSortLogRange | local;
+          if (count != nullptr) atomicAdd(count + local, 1);
+        }
+      len += __popc(m0) + __popc(m1);
     }
   }
-  __syncwarp();
+  return len;
+}
+
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
 }
 
 template <typename TI>
 __global__ void __launch_bounds__(kSortWarps * 32, 1)
-    embed_sort_kernel(const TI* __restrict__ ids, int n, int vocab, long long padding, int range, EmbedWs ws,
-                      long long counters, int* __restrict__ status) {
-  extern __shared__ int sm[];  // [kSortWarps][range] counters, [kSortWarps][2][kSortList] matches
-  __shared__ int s_less[kSortWarps];
-  __shared__ int s_sum[kSortWarps];
+    embed_sort_kernel(const TI* __restrict__ ids, int n, int per, unsigned vocab, unsigned padding, EmbedWs ws,
+                      int* __restrict__ status) {
+  // [kSortWarps][per] tokens of each warp, [kSortWarps][range] offsets of each ranking warp
+  extern __shared__ int sm[];
+  __shared__ int s_count[1 << kSortLogRange];  // tokens of each local id, then its next position
+  __shared__ int s_less[kSortWarps], s_len[kSortWarps], s_sum[kSortWarps], s_off[kSortWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int* hist = sm + warp * range;
-  int* list_tok = sm + kSortWarps * range + warp * 2 * kSortList;
-  int* list_id = list_tok + kSortList;
-  const int lo = blockIdx.x * range;
-  const int width = min(range, vocab - lo);
-  for (int i = lane; i < range; i += 32) hist[i] = 0;
+  const int range = 1 << ws.log_r;
+  const int cta = blockIdx.x;
+  const int segment = kSortWarps * per;  // tokens whose lists fit into shared memory
+  int* list = sm + warp * per;
+  int* hist = sm + kSortWarps * per;
+  if (threadIdx.x < range) s_count[threadIdx.x] = 0;
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < counters;
-       i += static_cast<long long>(gridDim.x) * blockDim.x)
-    ws.count[i] = 0;
-  __syncwarp();
-  const int per = ((n + kSortWarps - 1) / kSortWarps + 31) & ~31;
-  const int beg = static_cast<int>(min(static_cast<long long>(warp) * per, static_cast<long long>(n)));
-  const int end = static_cast<int>(min(static_cast<long long>(beg) + per, static_cast<long long>(n)));
+  const bool wide = reinterpret_cast<uintptr_t>(ids) % (2 * sizeof(TI)) == 0;
   int len = 0, less = 0;
-  bool bad = false, spilled = false;
-  auto count = [&](const int* tok, const int* id, int i, int m) {
-    const bool on = i + lane < m;
-    const int k = on ? id[i + lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, k);
-    if (on && (same & ((1u << lane) - 1)) == 0) hist[k] += __popc(same);
-    __syncwarp();
-  };
-  sweep(ids, beg, end, vocab, padding, lo, width, lane, list_tok, list_id, len, less, bad, spilled, count);
-  for (int i = 0; i < len; i += 32) count(list_tok, list_id, i, len);
+  bool bad = false;
+  for (int seg = 0; seg < n; seg += segment) {
+    const int beg = min(n, seg + warp * per);
+    len = sweep(ids, seg, beg, min(n, beg + per), wide, vocab, padding, cta, ws.log_c, lane, list, s_count, less, bad);
+  }
   if (blockIdx.x == 0 && bad) atomicOr(status, kStatusBadShape);
   less = warp_sum(less);
-  if (lane == 0) s_less[warp] = less;
-  __syncthreads();
-  // thread j: the warps' counts of id lo + j become offsets; a block scan over j gives the starts
-  const int j = threadIdx.x;
-  int total = 0;
-  if (j < width)
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = sm[w * range + j];
-      sm[w * range + j] = total;
-      total += c;
-    }
-  int incl = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
+  if (lane == 0) {
+    s_less[warp] = less;
+    s_len[warp] = len;
   }
+  __syncthreads();
+  // first position of each local id: the tokens of earlier CTAs, and of smaller local ids
+  const int total = threadIdx.x < range ? s_count[threadIdx.x] : 0;
+  const int incl = warp_scan(total, lane);
   if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  int base = 0;
-  for (int w = 0; w < kSortWarps; ++w) {
-    base += s_less[w];
-    if (w < warp) base += s_sum[w];
+  const int base = warp_sum(s_less[lane]);
+  if (threadIdx.x < range) {
+    int first = base + incl - total;
+    for (int w = 0; w < warp; ++w) first += s_sum[w];
+    s_count[threadIdx.x] = first;
+    ws.start[cta * range + threadIdx.x] = first;
+    if (cta == gridDim.x - 1 && threadIdx.x == range - 1) ws.start[ws.slots()] = first + total;
   }
-  const int first = base + incl - total;
-  if (j < width) {
-    ws.start[lo + j] = first;
-    if (lo + j == vocab - 1) ws.start[vocab] = first + total;
-    for (int w = 0; w < kSortWarps; ++w) sm[w * range + j] += first;
-  }
-  __syncthreads();
-  auto place = [&](const int* tok, const int* id, int i, int m) {
-    const bool on = i + lane < m;
-    const int k = on ? id[i + lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, k);
-    if (on) {
-      const int at = hist[k] + __popc(same & ((1u << lane) - 1));
-      ws.order[at] = tok[i + lane];
-      ws.key[at] = lo + k;
+  for (int seg = 0; seg < n; seg += segment) {
+    if (n > segment) {  // the lists hold the last segment only
+      __syncthreads();
+      const int beg = min(n, seg + warp * per);
+      len = sweep(ids, seg, beg, min(n, beg + per), wide, vocab, padding, cta, ws.log_c, lane, list, static_cast<int*>(nullptr),
+                  less, bad);
+      if (lane == 0) s_len[warp] = len;
+      __syncthreads();
     }
-    __syncwarp();
-    if (on && (same & ((1u << lane) - 1)) == 0) hist[k] += __popc(same);
-    __syncwarp();
-  };
-  if (spilled)
-    sweep(ids, beg, end, vocab, padding, lo, width, lane, list_tok, list_id, len, less, bad, spilled, place);
-  for (int i = 0; i < len; i += 32) place(list_tok, list_id, i, len);
+    // `rankers` warps share the segment's tokens, 64 or more each, in token order
+    const int mine = s_len[lane];
+    const int ends = warp_scan(mine, lane);
+    const int m = __shfl_sync(0xffffffffu, ends, 31);
+    const int rankers = max(1, min(kSortWarps, (m + 63) / 64));
+    const int share = ((m + rankers - 1) / rankers + 31) & ~31;
+    if (warp == 0) s_off[lane] = ends - mine;
+    for (int i = threadIdx.x; i < rankers * range; i += kSortWarps * 32) hist[i] = 0;
+    __syncthreads();
+    // item i of the segment lies in the last list that starts at or before i
+    auto item_at = [&](int i) {
+      int w = 0;
+#pragma unroll
+      for (int o = kSortWarps / 2; o > 0; o >>= 1)
+        if (s_off[w + o] <= i) w += o;
+      return sm[w * per + i - s_off[w]];
+    };
+    const int i0 = warp * share, i1 = min(m, i0 + share);
+    int* my = hist + warp * range;
+    constexpr int kLocal = (1 << kSortLogRange) - 1;
+    if (rankers > 1) {
+      for (int i = i0 + lane; i < i1; i += 32) atomicAdd(my + (item_at(i) & kLocal), 1);
+      __syncthreads();
+    }
+    if (threadIdx.x < range) {
+      int at = s_count[threadIdx.x];
+      if (rankers > 1) {
+        for (int w = 0; w < rankers; ++w) {
+          const int c = hist[w * range + threadIdx.x];
+          hist[w * range + threadIdx.x] = at;
+          at += c;
+        }
+        s_count[threadIdx.x] = at;
+      }
+    }
+    if (rankers > 1) __syncthreads();
+    else my = s_count;
+    for (int i = i0; i < i1; i += 32) {
+      const bool on = i + lane < i1;
+      const int item = on ? item_at(i + lane) : 0;
+      const int k = on ? item & kLocal : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, k);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      if (on) {
+        const int at = my[k] + rank;
+        ws.order[at] = seg + (static_cast<unsigned>(item) >> kSortLogRange);
+        ws.key[at] = cta * range + k;
+      }
+      __syncwarp();
+      if (on && rank == 0) my[k] += __popc(same);
+      __syncwarp();
+    }
+  }
 }
 
 // ------------------------------------------------------------------ backward: reduce
@@ -235,172 +307,200 @@ __device__ __forceinline__ void emit_row(float* __restrict__ dst, const float (&
   }
 }
 
-// part[slot][chunk] of `m` pieces, `step` chunks apart from chunk c0 on (the first in `slot0`,
-// the others in slot 0), added in order.
-template <int V>
-__device__ __forceinline__ void add_pieces(const float* part, long long chunks, int H, int col, int slot0, int c0, int m,
-                                           int step, float (&acc)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  constexpr int C = V < 4 ? V : 4;
-  for (int i0 = 0; i0 < m; i0 += 4) {
-    typename Pack<float, C>::Raw raw[4][V / C];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i0 + u < m) {
-        const long long c = c0 + static_cast<long long>(i0 + u) * step;
-        const float* p = part + ((i0 + u == 0 ? slot0 : 0) * chunks + c) * H + col;
-#pragma unroll
-        for (int q = 0; q < V / C; ++q)
-          raw[u][q] = __ldcg(reinterpret_cast<const typename Pack<float, C>::Raw*>(p + q * C));
-      }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i0 + u < m) {
-#pragma unroll
-        for (int q = 0; q < V / C; ++q) {
-          float t[C];
-          Pack<float, C>{raw[u][q]}.get(t);
-#pragma unroll
-          for (int j = 0; j < C; ++j) acc[q * C + j] += t[j];
-        }
-      }
-  }
-}
-
-// One piece of the run [s, e) lies in chunk c; its sum is already in `part`.  The warp that
-// delivers the run's last piece adds them all.
-template <int V>
-__device__ void join_run(EmbedWs ws, long long chunks, int H, int col, bool on, int lane, const int* counts_of_slab,
-                         int c, int s, int e, float* dst, float scale, int accumulate) {
-  int* cnt = const_cast<int*>(counts_of_slab);  // [3][chunks]
-  const int c0 = s / kChunk, c1 = (e - 1) / kChunk;
-  int m = c1 - c0 + 1, step = 1;
-  float acc[V];
-  if (m > kChunk) {  // groups of 32 pieces first
-    const int g = (c - c0) / kChunk;
-    const int gc = c0 + g * kChunk;
-    const int in_group = min(kChunk, m - g * kChunk);
-    int last = 0;
-    if (lane == 0) last = atomicAdd(cnt + (g == 0 ? 2 : 1) * chunks + gc, 1) == in_group - 1;
-    if (!__shfl_sync(0xffffffffu, last, 0)) return;
-    __threadfence();
-    __syncwarp();
-    if (on) {
-      add_pieces<V>(ws.part, chunks, H, col, g == 0 ? 1 : 0, gc, in_group, 1, acc);
-      store_f32<V>(ws.part + ((g == 0 ? 1 : 0) * chunks + gc) * H + col, acc);
-    }
-    __threadfence();
-    __syncwarp();
-    m = (m + kChunk - 1) / kChunk;
-    step = kChunk;
-  }
-  int last = 0;
-  if (lane == 0) last = atomicAdd(cnt + c0, 1) == m - 1;
-  if (!__shfl_sync(0xffffffffu, last, 0)) return;
-  __threadfence();
-  __syncwarp();
-  if (on) {
-    add_pieces<V>(ws.part, chunks, H, col, 1, c0, m, step, acc);
-    emit_row<V>(dst, acc, scale, accumulate);
-  }
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads)
-    embed_reduce_kernel(const T* __restrict__ dy, long long ldy, float* __restrict__ dw, long long ldw, EmbedWs ws,
+// A lane holds J vectors of V elements, 32 V columns apart: V J = kLaneColumns.
+template <typename T, int V, int J>
+__global__ void __launch_bounds__(kWarps * 32, 5)
+    embed_reduce_kernel(const T* __restrict__ dy, long long ldy, float* __restrict__ dw, long long ldw, EmbedWs ws, int n,
                         long long chunks, int slabs, int vocab, int H, float scale, int accumulate) {
+  __shared__ __align__(16) float s_head[kWarps][kSlab], s_tail[kWarps][kSlab];
+  __shared__ int s_flags[kWarps], s_id[kWarps];
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  if (task >= chunks * slabs) {  // rows that no token names
-    const long long r0 = (task - chunks * slabs) * kZeroRows;
-    if (accumulate || r0 >= vocab) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long chunk_ctas = chunks * slabs;
+  if (blockIdx.x >= chunk_ctas) {  // rows that no token names
+    const long long r0 = ((blockIdx.x - chunk_ctas) * kWarps + warp) * kZeroRows;
+    if (r0 >= vocab) return;
     const int rows = static_cast<int>(min(static_cast<long long>(kZeroRows), vocab - r0));
     bool empty = false;
-    if (lane < rows) empty = ws.start[r0 + lane] == ws.start[r0 + lane + 1];
+    if (lane < rows) {
+      const int slot = ws.slot_of(static_cast<int>(r0) + lane);
+      empty = ws.start[slot] == ws.start[slot + 1];
+    }
     const unsigned m = __ballot_sync(0xffffffffu, empty);
-    const float z[V] = {};
+    constexpr int C = V < 4 ? V : 4;
+    const float z[C] = {};
     for (int r = 0; r < rows; ++r)
       if (m >> r & 1)
-        for (int c = lane * V; c < H; c += 32 * V) store_f32<V>(dw + (r0 + r) * ldw + c, z);
+        for (int c = lane * C; c < H; c += 32 * C) store_f32<C>(dw + (r0 + r) * ldw + c, z);
     return;
   }
-  const int c = static_cast<int>(task / slabs);
-  const int slab = static_cast<int>(task - static_cast<long long>(c) * slabs);
-  const int valid = ws.start[vocab];
-  const int p0 = c * kChunk;
-  const int m = min(kChunk, valid - p0);
-  if (m <= 0) return;
-  const int col = (slab * 32 + lane) * V;
-  const bool on = col < H;
-  int tok = 0, key = -1;
-  if (lane < m) {
+  const int chunk = static_cast<int>(blockIdx.x / slabs);
+  const int slab = static_cast<int>(blockIdx.x - static_cast<long long>(chunk) * slabs);
+  const int p0 = chunk * kChunk + warp * kWarpTokens;
+  const int col0 = slab * kSlab;
+  const int col = col0 + lane * V;
+  bool on[J];
+#pragma unroll
+  for (int q = 0; q < J; ++q) on[q] = col + 32 * V * q < H;
+  // positions behind `valid` hold nothing: they are read with the rest and masked
+  const int valid = ws.start[ws.slots()];
+  int tok = 0, key = -1, before = -1, after = -1;
+  if (lane < kWarpTokens && p0 + lane < n) {
     tok = ws.order[p0 + lane];
     key = ws.key[p0 + lane];
   }
-  const int key0 = __shfl_sync(0xffffffffu, key, 0);
-  const int key1 = __shfl_sync(0xffffffffu, key, m - 1);
-  const int s0 = ws.start[key0], e0 = ws.start[key0 + 1];
-  const int s1 = ws.start[key1], e1 = ws.start[key1 + 1];
-  const bool head = s0 < p0;                          // the first run began in an earlier chunk
-  const bool tail = e1 > p0 + m && !(head && key0 == key1);  // the last run begins here and goes on
-  float acc[V];
+  if (p0 > 0 && p0 - 1 < n) before = ws.key[p0 - 1];
+  if (p0 + kWarpTokens < n) after = ws.key[p0 + kWarpTokens];
+  if (chunk * kChunk >= valid) return;  // the whole CTA
+  const int m = min(kWarpTokens, valid - p0);
+  if (p0 + kWarpTokens >= valid) after = -1;
+  int flags = 0, head_id = 0;  // 1: a run comes from before, 2: a run goes on behind, 4: it is one run
+  if (m > 0) {
+    Pack<T, V> x[kWarpTokens][J];
 #pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  int cur = key0;
-  bool first = head;
-  for (int i0 = 0; i0 < m; i0 += 8) {
-    Pack<T, V> x[8];
+    for (int u = 0; u < kWarpTokens; ++u) {
+      const long long t = __shfl_sync(0xffffffffu, tok, u);
+      if (u < m) {
+        const T* row = dy + t * ldy + col;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const long long t = __shfl_sync(0xffffffffu, tok, i0 + u);
-      if (i0 + u < m && on) x[u] = Pack<T, V>::load(dy + t * ldy + col);
+        for (int q = 0; q < J; ++q)
+          if (on[q]) x[u][q] = Pack<T, V>::load(row + 32 * V * q);
+      }
     }
+    const int key0 = __shfl_sync(0xffffffffu, key, 0), key1 = __shfl_sync(0xffffffffu, key, m - 1);
+    const bool head = before == key0, tail = after == key1;
+    flags = (head ? 1 : 0) | (tail ? 2 : 0) | (head && tail && key0 == key1 ? 4 : 0);
+    head_id = ws.id_of(key0);
+    // bit i: token i begins another run
+    const int up = __shfl_up_sync(0xffffffffu, key, 1);
+    const unsigned begins = __ballot_sync(0xffffffffu, lane > 0 && lane < m && key != up);
+    const int id = ws.id_of(key);
+    float acc[J][V];
+    auto clear = [&] {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int k = __shfl_sync(0xffffffffu, key, i0 + u);
-      if (i0 + u >= m) break;
-      if (k != cur) {
-        if (on) {
-          if (first) {
-            store_f32<V>(ws.part + static_cast<long long>(c) * H + col, acc);
-          } else {
-            emit_row<V>(dw + static_cast<long long>(cur) * ldw + col, acc, scale, accumulate);
-          }
+      for (int q = 0; q < J; ++q)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[q][j] = 0.f;
+    };
+    clear();
+    auto keep = [&](float* dst) {
+#pragma unroll
+      for (int q = 0; q < J; ++q) store_f32<V>(dst + (lane + 32 * q) * V, acc[q]);
+    };
+    bool first = head;
+    auto close = [&](int i) {  // the run that ends at token i
+      const long long r = __shfl_sync(0xffffffffu, id, i);
+      if (first) {
+        keep(s_head[warp]);
+      } else {
+        float* row = dw + r * ldw + col;
+#pragma unroll
+        for (int q = 0; q < J; ++q)
+          if (on[q]) emit_row<V>(row + 32 * V * q, acc[q], scale, accumulate);
+      }
+      first = false;
+    };
+#pragma unroll
+    for (int u = 0; u < kWarpTokens; ++u) {
+      if (u >= m) break;
+      if (begins >> u & 1) {
+        close(u - 1);
+        clear();
+      }
+#pragma unroll
+      for (int q = 0; q < J; ++q)
+        if (on[q]) {
+          float f[V];
+          x[u][q].get(f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[q][j] += f[j];
         }
-        first = false;
-        cur = k;
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    }
+    if (!first && tail) keep(s_tail[warp]);
+    else close(m - 1);
+  }
+  if (lane == 0) {
+    s_flags[warp] = flags;
+    s_id[warp] = head_id;
+  }
+  __syncthreads();
+  // Runs that cross warps: the threads of a column follow the one that is open.  What crosses the
+  // chunk's ends goes to the workspace.
+  for (int c = threadIdx.x; c < kSlab; c += kWarps * 32) {
+    if (col0 + c >= H) break;
+    float carry = 0.f;
+    bool from_before = s_flags[0] & 1, open = false;
+    for (int w = 0; w < kWarps; ++w) {
+      const int f = s_flags[w];
+      if (f & 1) {
+        carry += s_head[w][c];
+        open = f & 4;
+        if (!open) {
+          if (from_before) {
+            ws.part[static_cast<long long>(chunk) * H + col0 + c] = carry;
+          } else {
+            const float one[1] = {carry};
+            emit_row<1>(dw + s_id[w] * ldw + col0 + c, one, scale, accumulate);
+          }
+          from_before = false;
+        }
       }
-      if (on) {
-        float f[V];
-        x[u].get(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += f[j];
+      if ((f & 2) && !(f & 4)) {
+        carry = s_tail[w][c];
+        open = true;
+        from_before = false;
       }
     }
+    if (open) ws.part[((from_before ? 0 : chunks) + chunk) * H + col0 + c] = carry;
   }
-  if (on) {
-    if (first)
-      store_f32<V>(ws.part + static_cast<long long>(c) * H + col, acc);
-    else if (tail)
-      store_f32<V>(ws.part + (chunks + c) * H + col, acc);
-    else
-      emit_row<V>(dw + static_cast<long long>(cur) * ldw + col, acc, scale, accumulate);
+}
+
+// Runs that cross chunks: the CTA of the chunk where one begins adds its pieces, one per chunk; warp w
+// takes every eighth, then the warps in turn.
+__global__ void __launch_bounds__(kThreads)
+    embed_join_kernel(float* __restrict__ dw, long long ldw, EmbedWs ws, long long chunks, int slabs, int H, float scale,
+                      int accumulate) {
+  constexpr int kJoinWarps = kThreads / 32, B = 4;  // pieces in flight
+  static_assert(kThreads == kSlab, "a thread per column");
+  __shared__ float sum[kJoinWarps][kSlab];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = static_cast<int>(blockIdx.x / slabs);
+  const int col0 = static_cast<int>(blockIdx.x - static_cast<long long>(chunk) * slabs) * kSlab;
+  const int valid = ws.start[ws.slots()];
+  const int next = (chunk + 1) * kChunk;
+  const int slot = ws.key[next];  // there is a chunk behind this one
+  if (next >= valid || ws.key[next - 1] != slot) return;
+  const int s = ws.start[slot], e = ws.start[slot + 1];
+  if (s < next - kChunk) return;  // it began earlier
+  const int m = (e - 1) / kChunk - chunk + 1;
+  float acc[kLaneColumns];
+#pragma unroll
+  for (int j = 0; j < kLaneColumns; ++j) acc[j] = 0.f;
+  for (int i0 = warp; i0 < m; i0 += B * kJoinWarps) {
+    float x[B][kLaneColumns];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int i = i0 + u * kJoinWarps;
+      const float* p = ws.part + ((i == 0 ? chunks : 0) + chunk + i) * H + col0 + lane;  // the first lies in slot 1
+#pragma unroll
+      for (int j = 0; j < kLaneColumns; ++j) x[u][j] = i < m && col0 + lane + 32 * j < H ? p[32 * j] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < B; ++u)
+#pragma unroll
+      for (int j = 0; j < kLaneColumns; ++j) acc[j] += x[u][j];
   }
-  if (!head && !tail) return;
-  __threadfence();
-  __syncwarp();
-  const int* counts = ws.count + static_cast<long long>(slab) * 3 * chunks;
-  if (head)
-    join_run<V>(ws, chunks, H, col, on, lane, counts, c, s0, e0, dw + static_cast<long long>(key0) * ldw + col, scale,
-                accumulate);
-  if (tail)
-    join_run<V>(ws, chunks, H, col, on, lane, counts, c, s1, e1, dw + static_cast<long long>(key1) * ldw + col, scale,
-                accumulate);
+#pragma unroll
+  for (int j = 0; j < kLaneColumns; ++j) sum[warp][lane + 32 * j] = acc[j];
+  __syncthreads();
+  if (col0 + threadIdx.x >= H) return;
+  float v[1] = {0.f};
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) v[0] += sum[w][threadIdx.x];
+  emit_row<1>(dw + ws.id_of(slot) * ldw + col0 + threadIdx.x, v, scale, accumulate);
 }
 
 // ------------------------------------------------------------------ host
@@ -440,23 +540,23 @@ void by_float(at::ScalarType t, F&& f) {
 }
 
 long long align256(long long b) { return (b + 255) / 256 * 256; }
-int slab_columns(int v) { return 32 * v; }
 
 struct Plan {
-  int v, slabs;
-  long long chunks, counters;
-  long long off_order, off_key, off_count, off_part, bytes;
+  int v, slabs, log_c, log_r;
+  long long chunks, off_order, off_key, off_part, bytes;
 };
 Plan plan_bwd(long long n, long long vocab, int H, int v) {
   Plan p;
   p.v = v;
-  p.slabs = (H + slab_columns(v) - 1) / slab_columns(v);
+  p.slabs = (H + kSlab - 1) / kSlab;
+  p.log_c = 0;
+  while (p.log_c < kSortLogCtas && (1LL << p.log_c) < vocab) ++p.log_c;
+  p.log_r = 0;
+  while ((1LL << (p.log_c + p.log_r)) < vocab) ++(p.log_r < kSortLogRange ? p.log_r : p.log_c);
   p.chunks = (n + kChunk - 1) / kChunk;
-  p.counters = 3 * p.chunks * p.slabs;
-  p.off_order = align256((vocab + 1) * 4);
+  p.off_order = align256(((1LL << (p.log_c + p.log_r)) + 1) * 4);
   p.off_key = p.off_order + align256(n * 4);
-  p.off_count = p.off_key + align256(n * 4);
-  p.off_part = p.off_count + align256(p.counters * 4);
+  p.off_part = p.off_key + align256(n * 4);
   p.bytes = p.off_part + align256(2 * p.chunks * H * 4);
   return p;
 }
@@ -525,7 +625,7 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
   const long long n = ids.numel(), vocab = dw.size(0);
   REVPP_CHECK(dy.size(0) == n && dy.size(1) == dw.size(1), "dy must be [", n, ", ", dw.size(1), "], got [", dy.size(0),
               ", ", dy.size(1), "]");
-  REVPP_CHECK(n < (1LL << 30) && vocab < (1LL << 30) && dw.size(1) < (1LL << 30), "too many tokens, rows or columns");
+  REVPP_CHECK(n < (1LL << 26) && vocab < (1LL << 30) && dw.size(1) < (1LL << 30), "too many tokens, rows or columns");
   if (vocab == 0 || dw.size(1) == 0 || (n == 0 && accumulate)) return;
   check_same_device(dy, dw, "dy and dw");
   check_same_device(ids, dw, "ids and dw");
@@ -539,35 +639,39 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
   torch::Tensor buf = torch::empty({p.bytes}, dw.options().dtype(at::kByte));
   char* base = static_cast<char*>(buf.data_ptr());
   EmbedWs ws{reinterpret_cast<int*>(base), reinterpret_cast<int*>(base + p.off_order),
-             reinterpret_cast<int*>(base + p.off_key), reinterpret_cast<int*>(base + p.off_count),
-             reinterpret_cast<float*>(base + p.off_part)};
+             reinterpret_cast<int*>(base + p.off_key), reinterpret_cast<float*>(base + p.off_part), p.log_c, p.log_r};
   int* status = status_device_ptr();
-  const int range = static_cast<int>(
-      std::min<long long>(kSortRange, std::max<long long>(1, (vocab + num_sms() - 1) / num_sms())));
-  const int ctas = static_cast<int>((vocab + range - 1) / range);
-  const size_t smem = static_cast<size_t>(kSortWarps) * (range + 2 * kSortList) * 4;
+  // every warp lists a 32nd of the tokens, in segments of 32 x kSortPer where there are more
+  const int per = static_cast<int>(std::min<long long>(kSortPer, (n + kSortWarps * 64 - 1) / (kSortWarps * 64) * 64));
+  const size_t smem = static_cast<size_t>(kSortWarps) * ((1 << p.log_r) + per) * 4;
+  const unsigned padding = padding_idx >= 0 && padding_idx < vocab ? static_cast<unsigned>(padding_idx) : 0xffffffffu;
   auto sort = [&](auto ti) {
     using TI = decltype(ti);
-    REVPP_CUDA_CHECK(cudaFuncSetAttribute(embed_sort_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          kSortWarps * (kSortRange + 2 * kSortList) * 4));
-    launch_pdl(embed_sort_kernel<TI>, dim3(ctas), dim3(kSortWarps * 32), smem, cur_stream(),
-               static_cast<const TI*>(ids.data_ptr()), static_cast<int>(n), static_cast<int>(vocab),
-               static_cast<long long>(padding_idx), range, ws, p.counters, status);
+    static std::atomic<uint64_t> ready{0};  // devices that know the kernel's shared memory
+    const uint64_t bit = 1ull << (dw.get_device() & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+      REVPP_CUDA_CHECK(cudaFuncSetAttribute(embed_sort_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            kSortWarps * ((1 << kSortLogRange) + kSortPer) * 4));
+      ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    launch_pdl(embed_sort_kernel<TI>, dim3(1u << p.log_c), dim3(kSortWarps * 32), smem, cur_stream(),
+               static_cast<const TI*>(ids.data_ptr()), static_cast<int>(n), per, static_cast<unsigned>(vocab), padding, ws, status);
   };
   if (ids.scalar_type() == at::kLong) sort(int64_t{});
   else sort(int32_t{});
   REVPP_CHECK_LAUNCH();
-  const long long tasks = p.chunks * p.slabs + (accumulate ? 0 : (vocab + kZeroRows - 1) / kZeroRows);
-  const long long blocks = (tasks + kThreads / 32 - 1) / (kThreads / 32);
+  const long long zero_rows = kWarps * kZeroRows;
+  const long long blocks = p.chunks * p.slabs + (accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows);
   REVPP_CHECK(blocks < (1LL << 31), "too many tokens");
   by_float(dy.scalar_type(), [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto vc) {
       constexpr int V = decltype(vc)::value;
       if constexpr (V * sizeof(T) <= 16)
-        launch_pdl(embed_reduce_kernel<T, V>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, cur_stream(),
-                   static_cast<const T*>(dy.data_ptr()), static_cast<long long>(dy.stride(0)), dw.data_ptr<float>(),
-                   static_cast<long long>(dw.stride(0)), ws, p.chunks, p.slabs, static_cast<int>(vocab), H,
+        launch_pdl(embed_reduce_kernel<T, V, kLaneColumns / V>, dim3(static_cast<unsigned>(blocks)), dim3(kWarps * 32), 0,
+                   cur_stream(), static_cast<const T*>(dy.data_ptr()), static_cast<long long>(dy.stride(0)),
+                   dw.data_ptr<float>(), static_cast<long long>(dw.stride(0)), ws, static_cast<int>(n), p.chunks, p.slabs,
+                   static_cast<int>(vocab), H,
                    static_cast<float>(scale), accumulate ? 1 : 0);
     };
     if (v == 8) go(std::integral_constant<int, 8>{});
@@ -575,6 +679,11 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
     else if (v == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 1>{});
   });
+  REVPP_CHECK_LAUNCH();
+  if (p.chunks < 2) return;  // no run crosses chunks
+  launch_pdl(embed_join_kernel, dim3(static_cast<unsigned>((p.chunks - 1) * p.slabs)), dim3(kThreads), 0, cur_stream(),
+             dw.data_ptr<float>(), static_cast<long long>(dw.stride(0)), ws, p.chunks, p.slabs, H,
+             static_cast<float>(scale), accumulate ? 1 : 0);
   REVPP_CHECK_LAUNCH();
 }
 

@@ -10,12 +10,13 @@
 // itself.  Statistics, rotation and sums are fp32; the result is rounded once.  A position outside
 // the tables sets kStatusBadShape and leaves the row unrotated.
 //
-// A head belongs to G lanes (a power of two).  Each lane owns "units" of two vectors of V
-// elements: in the rotated part the two vectors that hold the two members of V pairs, so that the
-// rotation needs no exchange between lanes, and behind it two neighbouring vectors.  A lane keeps
-// its head and walks over the rows: norm weights and, in the backward pass, their gradients stay
-// in registers.
+// A head belongs to G lanes.  Each lane owns U "units" of two vectors of V elements: in the
+// rotated part the two vectors that hold the two members of V pairs, so that the rotation needs no
+// exchange between lanes, and behind it two neighbouring vectors.  A lane keeps its head and walks
+// over the rows, the next row's vectors in flight while it works on one: norm weights and, in the
+// backward pass, their gradients stay in registers.  Arithmetic runs on packed fp32 pairs.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "host.h"
@@ -40,7 +41,7 @@ struct QkArgs {
   int seq;
   int table_rows;
   int rows, heads, kv_heads, all_heads, dim, rot;
-  int units, log_g;          // units per head, lanes per head
+  int units, group, groups;  // units per head, lanes per head, heads per warp
   float eps, inv_dim;
   int* status;
 };
@@ -71,270 +72,422 @@ __device__ __forceinline__ void unit_at(int u, int dim, int rot, int& a, int& b,
   }
 }
 
-__device__ __forceinline__ long long position_of(const QkArgs& a, int row) {
-  if (a.pos == nullptr) return static_cast<unsigned>(row) % static_cast<unsigned>(a.seq);
-  return a.pos64 ? static_cast<const int64_t*>(a.pos)[row] : static_cast<const int32_t*>(a.pos)[row];
+// Packed arithmetic on neighbouring elements of arrays (V = 1: plain).
+template <int V>
+__device__ __forceinline__ void mul(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      f32x2_split(mul_f32x2(f32x2(a[j], a[j + 1]), f32x2(b[j], b[j + 1])), d[j], d[j + 1]);
+  } else {
+    d[0] = a[0] * b[0];
+  }
+}
+template <int V>
+__device__ __forceinline__ void scale(float (&d)[V], float s) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) f32x2_split(mul_f32x2(f32x2(d[j], d[j + 1]), f32x2_splat(s)), d[j], d[j + 1]);
+  } else {
+    d[0] *= s;
+  }
+}
+// d = a b + c
+template <int V>
+__device__ __forceinline__ void mad(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      f32x2_split(fma_f32x2(f32x2(a[j], a[j + 1]), f32x2(b[j], b[j + 1]), f32x2(c[j], c[j + 1])), d[j], d[j + 1]);
+  } else {
+    d[0] = fmaf(a[0], b[0], c[0]);
+  }
+}
+// d = a s + c
+template <int V>
+__device__ __forceinline__ void mad(float (&d)[V], const float (&a)[V], float s, const float (&c)[V]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      f32x2_split(fma_f32x2(f32x2(a[j], a[j + 1]), f32x2_splat(s), f32x2(c[j], c[j + 1])), d[j], d[j + 1]);
+  } else {
+    d[0] = fmaf(a[0], s, c[0]);
+  }
+}
+// sum += a b, in two running halves
+template <int V>
+__device__ __forceinline__ void dot(float (&sum)[2], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      f32x2_split(fma_f32x2(f32x2(a[j], a[j + 1]), f32x2(b[j], b[j + 1]), f32x2(sum[0], sum[1])), sum[0], sum[1]);
+  } else {
+    sum[0] = fmaf(a[0], b[0], sum[0]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void zero(float (&d)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) d[j] = 0.f;
+}
+
+// Cosines and sines of a unit's pairs: V of each, for the pairs inside its two vectors V / 2 and V / 2.
+template <int V, bool NEIGHBOURS>
+__device__ __forceinline__ void load_angles(const float* __restrict__ cos, const float* __restrict__ sin, int pair, bool second,
+                                            float (&c)[V], float (&s)[V]) {
+  if constexpr (NEIGHBOURS && V > 1) {
+    constexpr int P = V / 2;
+    float t[P];
+    load_f32<P>(cos + pair, t);
+#pragma unroll
+    for (int j = 0; j < P; ++j) c[j] = t[j];
+    load_f32<P>(sin + pair, t);
+#pragma unroll
+    for (int j = 0; j < P; ++j) s[j] = t[j];
+    if (second) load_f32<P>(cos + pair + P, t);
+#pragma unroll
+    for (int j = 0; j < P; ++j) c[P + j] = second ? t[j] : 1.f;  // the second vector may lie behind rot
+    if (second) load_f32<P>(sin + pair + P, t);
+#pragma unroll
+    for (int j = 0; j < P; ++j) s[P + j] = second ? t[j] : 0.f;
+  } else {
+    load_f32<V>(cos + pair, c);
+    load_f32<V>(sin + pair, s);
+  }
 }
 
 // Rotates the unit (xa, xb) by +angle (SIGN 1) or -angle (SIGN -1).
 template <int V, bool NEIGHBOURS, int SIGN>
-__device__ __forceinline__ void rotate(float (&xa)[V], float (&xb)[V], const float* __restrict__ cos,
-                                       const float* __restrict__ sin, int pair, int b, int rot) {
+__device__ __forceinline__ void rotate(float (&xa)[V], float (&xb)[V], const float (&c)[V], const float (&s)[V]) {
   if constexpr (NEIGHBOURS && V > 1) {
     constexpr int P = V / 2;
-    float c[P], s[P];
-    load_f32<P>(cos + pair, c);
-    load_f32<P>(sin + pair, s);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const float p = xa[2 * j], q = xa[2 * j + 1], n = SIGN * s[j];
       xa[2 * j] = p * c[j] - q * n;
       xa[2 * j + 1] = p * n + q * c[j];
-    }
-    if (b >= 0 && b < rot) {
-      load_f32<P>(cos + pair + P, c);
-      load_f32<P>(sin + pair + P, s);
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        const float p = xb[2 * j], q = xb[2 * j + 1], n = SIGN * s[j];
-        xb[2 * j] = p * c[j] - q * n;
-        xb[2 * j + 1] = p * n + q * c[j];
-      }
+      const float pb = xb[2 * j], qb = xb[2 * j + 1], nb = SIGN * s[P + j];
+      xb[2 * j] = pb * c[P + j] - qb * nb;
+      xb[2 * j + 1] = pb * nb + qb * c[P + j];
     }
   } else {
-    float c[V], s[V];
-    load_f32<V>(cos + pair, c);
-    load_f32<V>(sin + pair, s);
+    float ya[V], yb[V], m[V], n[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float p = xa[j], q = xb[j], n = SIGN * s[j];
-      xa[j] = p * c[j] - q * n;
-      xb[j] = p * n + q * c[j];
+      m[j] = -SIGN * s[j];
+      n[j] = SIGN * s[j];
+    }
+    mul<V>(ya, xa, c);
+    mul<V>(yb, xb, c);
+    mad<V>(ya, xb, m, ya);
+    mad<V>(yb, xa, n, yb);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      xa[j] = ya[j];
+      xb[j] = yb[j];
     }
   }
 }
 
 // The lane's place: its head, first row and row stride (rows advance by whole sets of heads).
 struct Place {
-  int head, row, stride, lane;
+  int head, row, stride, lane;  // row >= rows: nothing to do
+  unsigned slot;
 };
 __device__ __forceinline__ Place place_of(const QkArgs& a) {
-  const unsigned slot = (blockIdx.x * kThreads + threadIdx.x) >> a.log_g;
-  const unsigned slots = (gridDim.x * kThreads) >> a.log_g;
-  const unsigned stride = slots / a.all_heads;
+  const int lane = threadIdx.x & 31, sub = lane / a.group;
+  const unsigned warps = gridDim.x * (kThreads / 32);
+  const unsigned warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   Place p;
-  p.row = slot / a.all_heads;
-  p.head = slot - p.row * a.all_heads;
-  p.stride = stride;
-  if (p.row >= static_cast<int>(stride)) p.row = a.rows;  // a remainder that makes no whole set
-  p.lane = threadIdx.x & ((1 << a.log_g) - 1);
+  p.slot = warp * a.groups + sub;
+  p.stride = warps * a.groups / a.all_heads;
+  p.row = p.slot / a.all_heads;
+  p.head = p.slot - p.row * a.all_heads;
+  // lanes behind the last whole group, and slots that make no whole set of heads
+  if (sub >= a.groups || p.row >= p.stride) p.row = a.rows;
+  p.lane = lane - sub * a.group;
   return p;
 }
 
-__device__ __forceinline__ float group_sum(float v, int log_g) {
-  for (int o = (1 << log_g) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sum over a head's lanes, in every one of them.  FULL: the lanes are a power of two.
+template <bool FULL>
+__device__ __forceinline__ float group_sum(float v, const QkArgs& a, int lane) {
+  if (FULL) {
+    for (int o = a.group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  for (int n = a.group; n > 1;) {
+    const int half = (n + 1) >> 1;
+    const float up = __shfl_down_sync(0xffffffffu, v, half);
+    if (lane + half < n) v += up;
+    n = half;
+  }
+  return __shfl_sync(0xffffffffu, v, (threadIdx.x & 31) - lane);
 }
 
-template <typename T, int V, int U, bool NEIGHBOURS>
+// What a lane keeps: its units' columns, norm weights and first pairs.
+template <int V, int U, bool NEIGHBOURS, bool FULL>
+struct Lane {
+  int ca[U], cb[U], pair[U];
+  bool turn[U], second[U];
+  float wa[U][V], wb[U][V];
+  __device__ __forceinline__ bool has_a(int u) const { return FULL || ca[u] >= 0; }
+  __device__ __forceinline__ bool has_b(int u) const { return FULL || cb[u] >= 0; }
+  __device__ __forceinline__ Lane(const QkArgs& a, const Place& p, const float* w) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int unit = p.lane + u * a.group;
+      unit_at<V, NEIGHBOURS>(unit, a.dim, a.rot, ca[u], cb[u], turn[u], pair[u]);
+      if (!FULL && unit >= a.units) {
+        ca[u] = cb[u] = -1;
+        turn[u] = false;
+      }
+      second[u] = cb[u] >= 0 && cb[u] < a.rot;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        wa[u][j] = w != nullptr && has_a(u) ? __ldg(w + ca[u] + j) : 1.f;
+        wb[u][j] = w != nullptr && has_b(u) ? __ldg(w + cb[u] + j) : 1.f;
+      }
+    }
+  }
+};
+
+// A row's position: the table row, or -1 where there is none.
+struct Positions {
+  int at, step;
+  __device__ __forceinline__ Positions(const QkArgs& a, const Place& p) {
+    at = step = 0;
+    if (a.rot > 0 && a.pos == nullptr) {
+      at = static_cast<unsigned>(p.row) % static_cast<unsigned>(a.seq);
+      step = static_cast<unsigned>(p.stride) % static_cast<unsigned>(a.seq);
+    }
+  }
+  // of `row`; rows come in order
+  __device__ __forceinline__ long long next(const QkArgs& a, int row) {
+    if (a.pos != nullptr)
+      return a.pos64 ? static_cast<const int64_t*>(a.pos)[row] : static_cast<const int32_t*>(a.pos)[row];
+    const int now = at;
+    at += step;
+    if (at >= a.seq) at -= a.seq;
+    return now;
+  }
+};
+
+template <typename T, int V, int U>
+struct Vectors {
+  Pack<T, V> a[U], b[U];
+  template <typename L>
+  __device__ __forceinline__ void load(const T* p, const L& l) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (l.has_a(u)) a[u] = Pack<T, V>::load(p + l.ca[u]);
+      if (l.has_b(u)) b[u] = Pack<T, V>::load(p + l.cb[u]);
+    }
+  }
+  template <typename L>
+  __device__ __forceinline__ void store(T* p, const L& l) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (l.has_a(u)) a[u].store(p + l.ca[u]);
+      if (l.has_b(u)) b[u].store(p + l.cb[u]);
+    }
+  }
+  template <typename L>
+  __device__ __forceinline__ void get(float (&fa)[U][V], float (&fb)[U][V], const L& l) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (l.has_a(u)) a[u].get(fa[u]);
+      else zero<V>(fa[u]);
+      if (l.has_b(u)) b[u].get(fb[u]);
+      else zero<V>(fb[u]);
+    }
+  }
+};
+
+template <typename T, int V, int U, bool NEIGHBOURS, bool FULL>
 __global__ void __launch_bounds__(kThreads)
     qk_norm_rope_fwd_kernel(const T* x, T* y, QkArgs a) {
   pdl_wait();
   pdl_trigger();
   const Place p = place_of(a);
-  const int G = 1 << a.log_g;
   const bool norm = p.head < a.heads + a.kv_heads;
-  const float* w = p.head < a.heads ? a.wq : a.wk;
-  int ca[U], cb[U], pair[U];
-  bool turn[U];
-  float wa[U][V], wb[U][V];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int unit = p.lane + u * G;
-    unit_at<V, NEIGHBOURS>(unit, a.dim, a.rot, ca[u], cb[u], turn[u], pair[u]);
-    if (unit >= a.units) ca[u] = cb[u] = -1;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      wa[u][j] = norm && w != nullptr && ca[u] >= 0 ? __ldg(w + ca[u] + j) : 1.f;
-      wb[u][j] = norm && w != nullptr && cb[u] >= 0 ? __ldg(w + cb[u] + j) : 1.f;
-    }
-  }
+  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.head < a.heads ? a.wq : norm ? a.wk : nullptr);
+  Positions where(a, p);
+  const bool turns = norm && a.rot > 0;
+  const T* xr = x + static_cast<long long>(p.row) * a.ldx + p.head * a.dim;
+  T* yr = y + static_cast<long long>(p.row) * a.ldy + p.head * a.dim;
+  const long long step_x = static_cast<long long>(p.stride) * a.ldx, step_y = static_cast<long long>(p.stride) * a.ldy;
   const int trips = (a.rows + p.stride - 1) / p.stride;
-  for (int t = 0; t < trips; ++t) {
-    const int row = p.row + t * p.stride;
+  int row = p.row;
+  Vectors<T, V, U> now, next;
+  long long pos = -1, next_pos = -1;
+  if (row < a.rows) {
+    next.load(xr, l);
+    if (turns) next_pos = where.next(a, row);
+  }
+  for (int t = 0; t < trips; ++t, row += p.stride, yr += step_y) {
     const bool on = row < a.rows;
-    const T* xr = x + static_cast<long long>(row) * a.ldx + p.head * a.dim;
-    T* yr = y + static_cast<long long>(row) * a.ldy + p.head * a.dim;
-    Pack<T, V> ra[U], rb[U];
+    now = next;
+    pos = next_pos;
+    xr += step_x;
+    if (row + p.stride < a.rows) {
+      next.load(xr, l);
+      if (turns) next_pos = where.next(a, row + p.stride);
+    }
+    if (turns && on && (pos < 0 || pos >= a.table_rows)) {
+      atomicOr(a.status, kStatusBadShape);
+      pos = -1;
+    }
+    float c[U][V], s[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (turns && on && pos >= 0 && l.turn[u])
+        load_angles<V, NEIGHBOURS>(a.cos + pos * a.ldt, a.sin + pos * a.ldt, l.pair[u], l.second[u], c[u], s[u]);
+    float fa[U][V], fb[U][V], ss[2] = {0.f, 0.f};
+    now.get(fa, fb, l);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (on && ca[u] >= 0) ra[u] = Pack<T, V>::load(xr + ca[u]);
-      if (on && cb[u] >= 0) rb[u] = Pack<T, V>::load(xr + cb[u]);
+      dot<V>(ss, fa[u], fa[u]);
+      dot<V>(ss, fb[u], fb[u]);
     }
-    long long pos = -1;
-    if (on && norm && a.rot > 0) {
-      pos = position_of(a, row);
-      if (pos < 0 || pos >= a.table_rows) {
-        atomicOr(a.status, kStatusBadShape);
-        pos = -1;
-      }
-    }
-    float fa[U][V], fb[U][V], ss = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (on && ca[u] >= 0) {
-        ra[u].get(fa[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) fa[u][j] = 0.f;
-      }
-      if (on && cb[u] >= 0) {
-        rb[u].get(fb[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) fb[u][j] = 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) ss += fa[u][j] * fa[u][j] + fb[u][j] * fb[u][j];
-    }
-    const float r = rsqrtf(group_sum(ss, a.log_g) * a.inv_dim + a.eps);
+    const float r = rsqrtf(group_sum<FULL>(on ? ss[0] + ss[1] : 0.f, a, p.lane) * a.inv_dim + a.eps);
     if (!on) continue;
+    if (norm) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ca[u] < 0) continue;
-      if (norm) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          fa[u][j] *= r * wa[u][j];
-          fb[u][j] *= r * wb[u][j];
-        }
-        if (turn[u] && pos >= 0)
-          rotate<V, NEIGHBOURS, 1>(fa[u], fb[u], a.cos + pos * a.ldt, a.sin + pos * a.ldt, pair[u], cb[u], a.rot);
-        ra[u].set(fa[u]);
-        rb[u].set(fb[u]);
+      for (int u = 0; u < U; ++u) {
+        mul<V>(fa[u], fa[u], l.wa[u]);
+        mul<V>(fb[u], fb[u], l.wb[u]);
+        scale<V>(fa[u], r);
+        scale<V>(fb[u], r);
+        if (turns && pos >= 0 && l.turn[u]) rotate<V, NEIGHBOURS, 1>(fa[u], fb[u], c[u], s[u]);
+        now.a[u].set(fa[u]);
+        now.b[u].set(fb[u]);
       }
-      ra[u].store(yr + ca[u]);
-      if (cb[u] >= 0) rb[u].store(yr + cb[u]);
     }
+    now.store(yr, l);
   }
 }
 
 // part: [gridDim.x][2][dim] sums of dz x r over the block's query heads and key heads, added up
 // by qk_weight_grad_kernel in block order.
-template <typename T, int V, int U, bool NEIGHBOURS>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int V, int U, bool NEIGHBOURS, bool FULL>
+__global__ void __launch_bounds__(kThreads, 2)
     qk_norm_rope_bwd_kernel(const T* dy, const T* __restrict__ x, T* dx, QkArgs a, float* __restrict__ part) {
-  extern __shared__ float sums[];  // [kThreads / G][dim]
+  extern __shared__ float sums[];  // [heads in the block][dim]
   pdl_wait();
   pdl_trigger();
   const Place p = place_of(a);
-  const int G = 1 << a.log_g;
   const bool norm = p.head < a.heads + a.kv_heads;
-  const float* w = p.head < a.heads ? a.wq : a.wk;
-  int ca[U], cb[U], pair[U];
-  bool turn[U];
-  float wa[U][V], wb[U][V], da[U][V], db[U][V];
+  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.head < a.heads ? a.wq : norm ? a.wk : nullptr);
+  Positions where(a, p);
+  const bool turns = norm && a.rot > 0;
+  const int col = p.head * a.dim;
+  const T* xr = x + static_cast<long long>(p.row) * a.ldx + col;
+  const T* gr = dy + static_cast<long long>(p.row) * a.ldy + col;
+  T* dr = dx + static_cast<long long>(p.row) * a.lddx + col;
+  const long long step_x = static_cast<long long>(p.stride) * a.ldx, step_g = static_cast<long long>(p.stride) * a.ldy,
+                  step_d = static_cast<long long>(p.stride) * a.lddx;
+  float da[U][V], db[U][V];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int unit = p.lane + u * G;
-    unit_at<V, NEIGHBOURS>(unit, a.dim, a.rot, ca[u], cb[u], turn[u], pair[u]);
-    if (unit >= a.units) ca[u] = cb[u] = -1;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      wa[u][j] = norm && w != nullptr && ca[u] >= 0 ? __ldg(w + ca[u] + j) : 1.f;
-      wb[u][j] = norm && w != nullptr && cb[u] >= 0 ? __ldg(w + cb[u] + j) : 1.f;
-      da[u][j] = db[u][j] = 0.f;
-    }
+    zero<V>(da[u]);
+    zero<V>(db[u]);
   }
   const int trips = (a.rows + p.stride - 1) / p.stride;
-  for (int t = 0; t < trips; ++t) {
-    const int row = p.row + t * p.stride;
+  int row = p.row;
+  Vectors<T, V, U> now_x, next_x, now_g, next_g;
+  long long pos = -1, next_pos = -1;
+  if (row < a.rows) {
+    next_g.load(gr, l);
+    if (norm) next_x.load(xr, l);
+    if (turns) next_pos = where.next(a, row);
+  }
+  for (int t = 0; t < trips; ++t, row += p.stride, dr += step_d) {
     const bool on = row < a.rows;
-    const bool work = on && norm;
-    const T* xr = x + static_cast<long long>(row) * a.ldx + p.head * a.dim;
-    const T* gr = dy + static_cast<long long>(row) * a.ldy + p.head * a.dim;
-    T* dr = dx + static_cast<long long>(row) * a.lddx + p.head * a.dim;
-    Pack<T, V> ra[U], rb[U], ga[U], gb[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (on && ca[u] >= 0) ga[u] = Pack<T, V>::load(gr + ca[u]);
-      if (on && cb[u] >= 0) gb[u] = Pack<T, V>::load(gr + cb[u]);
-      if (work && ca[u] >= 0) ra[u] = Pack<T, V>::load(xr + ca[u]);
-      if (work && cb[u] >= 0) rb[u] = Pack<T, V>::load(xr + cb[u]);
+    now_x = next_x;
+    now_g = next_g;
+    pos = next_pos;
+    xr += step_x;
+    gr += step_g;
+    if (row + p.stride < a.rows) {
+      next_g.load(gr, l);
+      if (norm) next_x.load(xr, l);
+      if (turns) next_pos = where.next(a, row + p.stride);
     }
-    long long pos = -1;
-    if (work && a.rot > 0) {
-      pos = position_of(a, row);
-      if (pos < 0 || pos >= a.table_rows) {
-        atomicOr(a.status, kStatusBadShape);
-        pos = -1;
-      }
+    if (turns && on && (pos < 0 || pos >= a.table_rows)) {
+      atomicOr(a.status, kStatusBadShape);
+      pos = -1;
     }
-    float xa[U][V], xb[U][V], za[U][V], zb[U][V], ss = 0.f, dot = 0.f;
+    float xa[U][V], xb[U][V], za[U][V], zb[U][V], ss[2] = {0.f, 0.f}, gx[2] = {0.f, 0.f};
+    if (on && norm) {
+      now_x.get(xa, xb, l);
+      now_g.get(za, zb, l);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) xa[u][j] = xb[u][j] = za[u][j] = zb[u][j] = 0.f;
-      if (work && ca[u] >= 0) {
-        ra[u].get(xa[u]);
-        ga[u].get(za[u]);
-      }
-      if (work && cb[u] >= 0) {
-        rb[u].get(xb[u]);
-        gb[u].get(zb[u]);
-      }
-      if (turn[u] && pos >= 0 && ca[u] >= 0)
-        rotate<V, NEIGHBOURS, -1>(za[u], zb[u], a.cos + pos * a.ldt, a.sin + pos * a.ldt, pair[u], cb[u], a.rot);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        ss += xa[u][j] * xa[u][j] + xb[u][j] * xb[u][j];
-        dot += za[u][j] * wa[u][j] * xa[u][j] + zb[u][j] * wb[u][j] * xb[u][j];
-      }
-    }
-    const float r = rsqrtf(group_sum(ss, a.log_g) * a.inv_dim + a.eps);
-    dot = group_sum(dot, a.log_g) * a.inv_dim * r * r;  // mean(g x r) r
-    if (!on) continue;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ca[u] < 0) continue;
-      if (norm) {
-        float oa[V], ob[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          da[u][j] += za[u][j] * (xa[u][j] * r);
-          db[u][j] += zb[u][j] * (xb[u][j] * r);
-          oa[j] = r * (za[u][j] * wa[u][j] - xa[u][j] * dot);
-          ob[j] = r * (zb[u][j] * wb[u][j] - xb[u][j] * dot);
+      for (int u = 0; u < U; ++u) {
+        if (turns && pos >= 0 && l.turn[u]) {
+          float c[V], s[V];
+          load_angles<V, NEIGHBOURS>(a.cos + pos * a.ldt, a.sin + pos * a.ldt, l.pair[u], l.second[u], c, s);
+          rotate<V, NEIGHBOURS, -1>(za[u], zb[u], c, s);
         }
-        ga[u].set(oa);
-        gb[u].set(ob);
+        dot<V>(ss, xa[u], xa[u]);
+        dot<V>(ss, xb[u], xb[u]);
+        float t_[V];
+        mul<V>(t_, xa[u], l.wa[u]);
+        dot<V>(gx, za[u], t_);
+        mul<V>(t_, xb[u], l.wb[u]);
+        dot<V>(gx, zb[u], t_);
       }
-      ga[u].store(dr + ca[u]);
-      if (cb[u] >= 0) gb[u].store(dr + cb[u]);
     }
+    const float r = rsqrtf(group_sum<FULL>(ss[0] + ss[1], a, p.lane) * a.inv_dim + a.eps);
+    const float mean = group_sum<FULL>(gx[0] + gx[1], a, p.lane) * a.inv_dim * r * r;  // mean(g x r) r
+    if (!on) continue;
+    if (norm) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float t_[V];
+        // dw += dz (x r);  dx = r (dz w - x mean)
+        mul<V>(t_, za[u], xa[u]);
+        mad<V>(da[u], t_, r, da[u]);
+        mul<V>(t_, zb[u], xb[u]);
+        mad<V>(db[u], t_, r, db[u]);
+        mul<V>(za[u], za[u], l.wa[u]);
+        mul<V>(zb[u], zb[u], l.wb[u]);
+        mad<V>(za[u], xa[u], -mean, za[u]);
+        mad<V>(zb[u], xb[u], -mean, zb[u]);
+        scale<V>(za[u], r);
+        scale<V>(zb[u], r);
+        now_g.a[u].set(za[u]);
+        now_g.b[u].set(zb[u]);
+      }
+    }
+    now_g.store(dr, l);
   }
   if (part == nullptr) return;
-  const int groups = kThreads >> a.log_g;
-  float* mine = sums + (threadIdx.x >> a.log_g) * a.dim;
+  const int heads = a.groups * (kThreads / 32);  // of the block
+  const int sub = (threadIdx.x & 31) / a.group;
+  if (sub < a.groups) {
+    float* mine = sums + ((threadIdx.x >> 5) * a.groups + sub) * a.dim;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (ca[u] >= 0) mine[ca[u] + j] = da[u][j];
-      if (cb[u] >= 0) mine[cb[u] + j] = db[u][j];
-    }
+      for (int j = 0; j < V; ++j) {
+        if (l.has_a(u)) mine[l.ca[u] + j] = da[u][j];
+        if (l.has_b(u)) mine[l.cb[u] + j] = db[u][j];
+      }
+  }
   __syncthreads();
-  const unsigned slot0 = (blockIdx.x * kThreads) >> a.log_g;
+  const unsigned slot0 = blockIdx.x * heads;
   for (int c = threadIdx.x; c < 2 * a.dim; c += kThreads) {
     const bool keys = c >= a.dim;
-    const int col = keys ? c - a.dim : c;
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) {
-      const int head = (slot0 + g) % a.all_heads;
+    const int column = keys ? c - a.dim : c;
+    float v = 0.f;
+    int head = slot0 % a.all_heads;
+    for (int g = 0; g < heads; ++g) {
       const bool use = keys ? head >= a.heads && head < a.heads + a.kv_heads : head < a.heads;
-      if (use) s += sums[g * a.dim + col];
+      if (use) v += sums[g * a.dim + column];
+      if (++head == a.all_heads) head = 0;
     }
-    part[static_cast<long long>(blockIdx.x) * 2 * a.dim + c] = s;
+    part[static_cast<long long>(blockIdx.x) * 2 * a.dim + c] = v;
   }
 }
 
@@ -391,7 +544,8 @@ void check_packed(const torch::Tensor& t, const char* name, int64_t rows, int64_
 
 struct Problem {
   QkArgs a;
-  int v;
+  int v, u;
+  bool full;
 };
 
 // Checks that need no device, then fills in the arguments.
@@ -479,7 +633,13 @@ void finish(Problem& p, std::initializer_list<const torch::Tensor*> packed, cons
     a.units = (a.dim / v + 1) / 2;
   else
     a.units = half / v + ((a.dim - a.rot) / v + 1) / 2;
-  while (a.log_g < 5 && (1 << a.log_g) < a.units) ++a.log_g;
+  // One unit per lane, or (narrow vectors) as many as leave fewer lanes idle; heads do not cross warps.
+  auto lanes = [&](int u) { return (a.units + u - 1) / u; };
+  p.u = v == 2 ? 2 : v == 1 ? 4 : 1;
+  if (lanes(1) <= 32 && (p.u == 1 || (32 / lanes(1)) * p.u >= 32 / lanes(p.u))) p.u = 1;
+  a.group = lanes(p.u);
+  a.groups = 32 / a.group;
+  p.full = v * size == 16 && 2 * v * a.units == a.dim && (a.group & (a.group - 1)) == 0;
   a.wq = given(wq) ? wq->data_ptr<float>() : nullptr;
   a.wk = given(wk) ? wk->data_ptr<float>() : nullptr;
   if (a.rot > 0) {
@@ -497,27 +657,47 @@ void finish(Problem& p, std::initializer_list<const torch::Tensor*> packed, cons
   a.status = status_device_ptr();
 }
 
+constexpr int kMaxSmem = 16 << 10;  // of the weight gradients: 8 warps x 2 x 8 x 32 columns at most
+
+// Blocks of a kernel that fit on an SM of the current device.
+template <auto Kernel>
+int resident(int device) {
+  static std::atomic<int> known[64];
+  std::atomic<int>& k = known[device & 63];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    REVPP_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, kThreads, kMaxSmem));
+    n = std::max(1, n);
+    k.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 // Blocks for one resident wave, or fewer when the rows need fewer.
-template <typename K>
-int blocks_for(K kernel, const QkArgs& a, size_t smem) {
-  int per_sm = 0;
-  REVPP_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem));
-  const long long need = ((static_cast<long long>(a.rows) * a.all_heads << a.log_g) + kThreads - 1) / kThreads;
-  const long long least = ((static_cast<long long>(a.all_heads) << a.log_g) + kThreads - 1) / kThreads;
-  const long long wave = static_cast<long long>(std::max(1, per_sm)) * num_sms();
+template <auto Kernel>
+int blocks_for(const QkArgs& a, int device) {
+  const int per_block = a.groups * (kThreads / 32);
+  const long long need = (static_cast<long long>(a.rows) * a.all_heads + per_block - 1) / per_block;
+  const long long least = (a.all_heads + per_block - 1) / per_block;
+  const long long wave = static_cast<long long>(resident<Kernel>(device)) * num_sms();
   return static_cast<int>(std::max(least, std::min(need, wave)));
 }
 
 template <typename F>
 void by_type(const Problem& p, at::ScalarType t, bool interleaved, F&& f) {
+  using std::integral_constant;
   auto by_v = [&](auto e, auto nb) {
     using T = decltype(e);
-    if constexpr (sizeof(T) == 2) {
-      if (p.v == 8) return f(e, std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}, nb);
+    constexpr int W = 16 / sizeof(T);
+    if (p.v == W && p.full) return f(e, integral_constant<int, W>{}, integral_constant<int, 1>{}, nb, std::true_type{});
+    if (p.v == W) return f(e, integral_constant<int, W>{}, integral_constant<int, 1>{}, nb, std::false_type{});
+    if constexpr (W > 4) {
+      if (p.v == 4) return f(e, integral_constant<int, 4>{}, integral_constant<int, 1>{}, nb, std::false_type{});
     }
-    if (p.v == 4) f(e, std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{}, nb);
-    else if (p.v == 2) f(e, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}, nb);
-    else f(e, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, nb);
+    if (p.v == 2 && p.u == 1) return f(e, integral_constant<int, 2>{}, integral_constant<int, 1>{}, nb, std::false_type{});
+    if (p.v == 2) return f(e, integral_constant<int, 2>{}, integral_constant<int, 2>{}, nb, std::false_type{});
+    if (p.u == 1) return f(e, integral_constant<int, 1>{}, integral_constant<int, 1>{}, nb, std::false_type{});
+    f(e, integral_constant<int, 1>{}, integral_constant<int, 4>{}, nb, std::false_type{});
   };
   auto by_pairs = [&](auto e) {
     if (interleaved) by_v(e, std::true_type{});
@@ -543,10 +723,11 @@ void qk_norm_rope_fwd(const torch::Tensor& qkv, torch::Tensor out, int64_t heads
   QkArgs& a = p.a;
   a.ldy = out.stride(0);
   a.all_heads = a.heads + a.kv_heads * (qkv.data_ptr() == out.data_ptr() ? 1 : 2);
-  by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb) {
+  by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb, auto full) {
     using T = decltype(e);
-    auto kernel = qk_norm_rope_fwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value>;
-    launch_pdl(kernel, dim3(blocks_for(kernel, a, 0)), dim3(kThreads), 0, cur_stream(),
+    constexpr auto kernel =
+        &qk_norm_rope_fwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value, decltype(full)::value>;
+    launch_pdl(kernel, dim3(blocks_for<kernel>(a, qkv.get_device())), dim3(kThreads), 0, cur_stream(),
                static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(out.data_ptr()), a);
   });
   REVPP_CHECK_LAUNCH();
@@ -585,11 +766,13 @@ void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch
     a.ldy = dout.stride(0);
     a.lddx = dqkv.stride(0);
     a.all_heads = a.heads + a.kv_heads * (dout.data_ptr() == dqkv.data_ptr() ? 1 : 2);
-    const size_t smem = weights ? static_cast<size_t>(kThreads >> a.log_g) * a.dim * 4 : 0;
-    by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb) {
+    const size_t smem = weights ? static_cast<size_t>(kThreads / 32) * a.groups * a.dim * 4 : 0;
+    REVPP_CHECK(smem <= kMaxSmem, "shared memory");
+    by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb, auto full) {
       using T = decltype(e);
-      auto kernel = qk_norm_rope_bwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value>;
-      blocks = blocks_for(kernel, a, smem);
+      constexpr auto kernel =
+          &qk_norm_rope_bwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value, decltype(full)::value>;
+      blocks = blocks_for<kernel>(a, qkv.get_device());
       if (weights) part = torch::empty({static_cast<int64_t>(blocks) * 2 * a.dim}, qkv.options().dtype(at::kFloat));
       launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, cur_stream(), static_cast<const T*>(dout.data_ptr()),
                  static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(dqkv.data_ptr()), a,
