@@ -12,9 +12,13 @@
 //
 // A head belongs to G lanes.  Each lane owns U "units" of two vectors of V elements: in the
 // rotated part the two vectors that hold the two members of V pairs, so that the rotation needs no
-// exchange between lanes, and behind it two neighbouring vectors.  A lane keeps its head and walks
-// over the rows, the next row's vectors in flight while it works on one: norm weights and, in the
-// backward pass, their gradients stay in registers.  Arithmetic runs on packed fp32 pairs.
+// exchange between lanes, and behind it two neighbouring vectors.  A lane keeps its head or heads and
+// walks over the rows: norm weights and, in the backward pass, their gradients stay in registers.
+// Arithmetic runs on packed fp32 pairs.  What bounds both passes is the number of bytes in flight:
+//  - fwd: a lane takes H heads of one kind (queries, keys or values) of a row, all loaded at once,
+//    with one set of angles;
+//  - bwd: one head, its vectors copied into shared memory two rows ahead (cp.async, every lane its
+//    own, so no barrier), since the registers are taken by weights and their gradients.
 #include <algorithm>
 #include <atomic>
 
@@ -28,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
+constexpr int kFwdHeads = 4;                  // heads that a lane of the forward pass has in flight
 
 struct QkArgs {
   long long ldx, ldy, lddx;  // row strides (elements)
@@ -40,7 +45,9 @@ struct QkArgs {
   int pos64;
   int seq;
   int table_rows;
-  int rows, heads, kv_heads, all_heads, dim, rot;
+  int rows, heads, kv_heads, dim, rot;
+  int q_sets, sets;          // sets of heads that a lane takes together: of queries, and of keys behind them
+  int copies;                // the value heads go to another buffer
   int units, group, groups;  // units per head, lanes per head, heads per warp
   float eps, inv_dim;
   int* status;
@@ -189,40 +196,48 @@ __device__ __forceinline__ void rotate(float (&xa)[V], float (&xb)[V], const flo
   }
 }
 
-// The lane's place: its head, first row and row stride (rows advance by whole sets of heads).
+// The lane's place: its heads, first row and row stride (rows advance by whole sets of heads).
 struct Place {
-  int head, row, stride, lane;  // row >= rows: nothing to do
-  unsigned slot;
+  bool keys;
+  int head, count;        // the first of `count` heads, among all of the row
+  int row, stride, lane;  // row >= rows: nothing to do
 };
+template <int H>
 __device__ __forceinline__ Place place_of(const QkArgs& a) {
   const int lane = threadIdx.x & 31, sub = lane / a.group;
   const unsigned warps = gridDim.x * (kThreads / 32);
   const unsigned warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   Place p;
-  p.slot = warp * a.groups + sub;
-  p.stride = warps * a.groups / a.all_heads;
-  p.row = p.slot / a.all_heads;
-  p.head = p.slot - p.row * a.all_heads;
+  const unsigned slot = warp * a.groups + sub;
+  p.stride = warps * a.groups / a.sets;
+  p.row = slot / a.sets;
+  const int set = slot - p.row * a.sets;
   // lanes behind the last whole group, and slots that make no whole set of heads
   if (sub >= a.groups || p.row >= p.stride) p.row = a.rows;
   p.lane = lane - sub * a.group;
+  p.keys = set >= a.q_sets;
+  const int first = (p.keys ? set - a.q_sets : set) * H;
+  p.head = first + (p.keys ? a.heads : 0);
+  p.count = min(H, (p.keys ? a.kv_heads : a.heads) - first);
   return p;
 }
 
-// Sum over a head's lanes, in every one of them.  FULL: the lanes are a power of two.
+// Sum over a head's lanes, in every one of them; the whole warp takes part.  FULL: the lanes are a
+// power of two.
 template <bool FULL>
-__device__ __forceinline__ float group_sum(float v, const QkArgs& a, int lane) {
-  if (FULL) {
+__device__ __forceinline__ float group_sum(float v, const QkArgs& a, const Place& p) {
+  if constexpr (FULL) {
     for (int o = a.group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+  } else {
+    for (int n = a.group; n > 1;) {
+      const int half = (n + 1) >> 1;
+      const float up = __shfl_down_sync(0xffffffffu, v, half);
+      if (p.lane + half < n) v += up;
+      n = half;
+    }
+    return __shfl_sync(0xffffffffu, v, (threadIdx.x & 31) - p.lane);
   }
-  for (int n = a.group; n > 1;) {
-    const int half = (n + 1) >> 1;
-    const float up = __shfl_down_sync(0xffffffffu, v, half);
-    if (lane + half < n) v += up;
-    n = half;
-  }
-  return __shfl_sync(0xffffffffu, v, (threadIdx.x & 31) - lane);
 }
 
 // What a lane keeps: its units' columns, norm weights and first pairs.
@@ -273,6 +288,13 @@ struct Positions {
   }
 };
 
+// The position, or -1 (and the status word set) for one outside the tables.
+__device__ __forceinline__ long long checked(const QkArgs& a, long long pos) {
+  if (pos >= 0 && pos < a.table_rows) return pos;
+  atomicOr(a.status, kStatusBadShape);
+  return -1;
+}
+
 template <typename T, int V, int U>
 struct Vectors {
   Pack<T, V> a[U], b[U];
@@ -304,83 +326,137 @@ struct Vectors {
   }
 };
 
-template <typename T, int V, int U, bool NEIGHBOURS, bool FULL>
-__global__ void __launch_bounds__(kThreads)
+// The value heads, once the lanes are through with queries and keys: a warp per row, four vectors of
+// every lane in flight.
+template <typename T, int V>
+__device__ __forceinline__ void copy_values(const T* src, long long ld_src, T* dst, long long ld_dst, const QkArgs& a) {
+  constexpr int B = 4;
+  const int first = (a.heads + a.kv_heads) * a.dim, width = a.kv_heads * a.dim;
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kThreads / 32);
+  for (int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); row < a.rows; row += warps) {
+    const T* s = src + row * ld_src + first;
+    T* d = dst + row * ld_dst + first;
+    for (int c0 = lane * V; c0 < width; c0 += 32 * V * B) {
+      Pack<T, V> v[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (c0 + 32 * V * i < width) v[i] = Pack<T, V>::load(s + c0 + 32 * V * i);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (c0 + 32 * V * i < width) v[i].store(d + c0 + 32 * V * i);
+    }
+  }
+}
+
+template <typename T, int V, int U, int H, bool NEIGHBOURS, bool FULL>
+__global__ void __launch_bounds__(kThreads, 2)
     qk_norm_rope_fwd_kernel(const T* x, T* y, QkArgs a) {
   pdl_wait();
   pdl_trigger();
-  const Place p = place_of(a);
-  const bool norm = p.head < a.heads + a.kv_heads;
-  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.head < a.heads ? a.wq : norm ? a.wk : nullptr);
+  const Place p = place_of<H>(a);
+  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.keys ? a.wk : a.wq);
   Positions where(a, p);
-  const bool turns = norm && a.rot > 0;
   const T* xr = x + static_cast<long long>(p.row) * a.ldx + p.head * a.dim;
   T* yr = y + static_cast<long long>(p.row) * a.ldy + p.head * a.dim;
   const long long step_x = static_cast<long long>(p.stride) * a.ldx, step_y = static_cast<long long>(p.stride) * a.ldy;
   const int trips = (a.rows + p.stride - 1) / p.stride;
   int row = p.row;
-  Vectors<T, V, U> now, next;
-  long long pos = -1, next_pos = -1;
-  if (row < a.rows) {
-    next.load(xr, l);
-    if (turns) next_pos = where.next(a, row);
-  }
-  for (int t = 0; t < trips; ++t, row += p.stride, yr += step_y) {
+  for (int t = 0; t < trips; ++t, row += p.stride, xr += step_x, yr += step_y) {
     const bool on = row < a.rows;
-    now = next;
-    pos = next_pos;
-    xr += step_x;
-    if (row + p.stride < a.rows) {
-      next.load(xr, l);
-      if (turns) next_pos = where.next(a, row + p.stride);
-    }
-    if (turns && on && (pos < 0 || pos >= a.table_rows)) {
-      atomicOr(a.status, kStatusBadShape);
-      pos = -1;
-    }
+    Vectors<T, V, U> v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (on && h < p.count) v[h].load(xr + h * a.dim, l);
+    const long long pos = on && a.rot > 0 ? checked(a, where.next(a, row)) : -1;
     float c[U][V], s[U][V];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (turns && on && pos >= 0 && l.turn[u])
+      if (pos >= 0 && l.turn[u])
         load_angles<V, NEIGHBOURS>(a.cos + pos * a.ldt, a.sin + pos * a.ldt, l.pair[u], l.second[u], c[u], s[u]);
-    float fa[U][V], fb[U][V], ss[2] = {0.f, 0.f};
-    now.get(fa, fb, l);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      dot<V>(ss, fa[u], fa[u]);
-      dot<V>(ss, fb[u], fb[u]);
-    }
-    const float r = rsqrtf(group_sum<FULL>(on ? ss[0] + ss[1] : 0.f, a, p.lane) * a.inv_dim + a.eps);
-    if (!on) continue;
-    if (norm) {
+    for (int h = 0; h < H; ++h) {
+      const bool here = on && h < p.count;
+      float fa[U][V], fb[U][V], ss[2] = {0.f, 0.f};
+      v[h].get(fa, fb, l);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        dot<V>(ss, fa[u], fa[u]);
+        dot<V>(ss, fb[u], fb[u]);
+      }
+      const float r = rsqrtf(group_sum<FULL>(here ? ss[0] + ss[1] : 0.f, a, p) * a.inv_dim + a.eps);
+      if (!here) continue;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         mul<V>(fa[u], fa[u], l.wa[u]);
         mul<V>(fb[u], fb[u], l.wb[u]);
         scale<V>(fa[u], r);
         scale<V>(fb[u], r);
-        if (turns && pos >= 0 && l.turn[u]) rotate<V, NEIGHBOURS, 1>(fa[u], fb[u], c[u], s[u]);
-        now.a[u].set(fa[u]);
-        now.b[u].set(fb[u]);
+        if (pos >= 0 && l.turn[u]) rotate<V, NEIGHBOURS, 1>(fa[u], fb[u], c[u], s[u]);
+        v[h].a[u].set(fa[u]);
+        v[h].b[u].set(fb[u]);
       }
+      v[h].store(yr + h * a.dim, l);
     }
-    now.store(yr, l);
+  }
+  if (a.copies) copy_values<T, V>(x, a.ldx, y, a.ldy, a);
+}
+
+// BYTES of global memory to shared memory, in the background from 4 bytes on.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  } else if constexpr (BYTES >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+  } else {
+    *static_cast<unsigned short*>(dst) = *static_cast<const unsigned short*>(src);
   }
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A thread's own ring of kStages rows: the vectors of dy and of x.
+constexpr int kStages = 3;
+template <typename T, int V, int U>
+struct Ring {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T)), kVectors = 4 * U;
+  static constexpr int kSize = kStages * kVectors * kThreads * kBytes;
+  char* base;
+  __device__ __forceinline__ T* at(int stage, int k) const {
+    return reinterpret_cast<T*>(base + ((stage * kVectors + k) * kThreads + threadIdx.x) * kBytes);
+  }
+  template <typename L>
+  __device__ __forceinline__ void fetch(int stage, int k0, const T* p, const L& l) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (l.has_a(u)) copy_async<kBytes>(at(stage, k0 + 2 * u), p + l.ca[u]);
+      if (l.has_b(u)) copy_async<kBytes>(at(stage, k0 + 2 * u + 1), p + l.cb[u]);
+    }
+  }
+  template <typename L>
+  __device__ __forceinline__ void read(Vectors<T, V, U>& v, int stage, int k0, const L& l) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (l.has_a(u)) v.a[u] = Pack<T, V>::load(at(stage, k0 + 2 * u));
+      if (l.has_b(u)) v.b[u] = Pack<T, V>::load(at(stage, k0 + 2 * u + 1));
+    }
+  }
+};
 
 // part: [gridDim.x][2][dim] sums of dz x r over the block's query heads and key heads, added up
 // by qk_weight_grad_kernel in block order.
 template <typename T, int V, int U, bool NEIGHBOURS, bool FULL>
 __global__ void __launch_bounds__(kThreads, 2)
     qk_norm_rope_bwd_kernel(const T* dy, const T* __restrict__ x, T* dx, QkArgs a, float* __restrict__ part) {
-  extern __shared__ float sums[];  // [heads in the block][dim]
+  extern __shared__ __align__(16) char shared[];  // the rings, then [sets in the block][dim] sums
   pdl_wait();
   pdl_trigger();
-  const Place p = place_of(a);
-  const bool norm = p.head < a.heads + a.kv_heads;
-  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.head < a.heads ? a.wq : norm ? a.wk : nullptr);
+  const Place p = place_of<1>(a);
+  const Lane<V, U, NEIGHBOURS, FULL> l(a, p, p.keys ? a.wk : a.wq);
   Positions where(a, p);
-  const bool turns = norm && a.rot > 0;
   const int col = p.head * a.dim;
   const T* xr = x + static_cast<long long>(p.row) * a.ldx + col;
   const T* gr = dy + static_cast<long long>(p.row) * a.ldy + col;
@@ -393,77 +469,84 @@ __global__ void __launch_bounds__(kThreads, 2)
     zero<V>(da[u]);
     zero<V>(db[u]);
   }
-  const int trips = (a.rows + p.stride - 1) / p.stride;
-  int row = p.row;
-  Vectors<T, V, U> now_x, next_x, now_g, next_g;
-  long long pos = -1, next_pos = -1;
-  if (row < a.rows) {
-    next_g.load(gr, l);
-    if (norm) next_x.load(xr, l);
-    if (turns) next_pos = where.next(a, row);
-  }
-  for (int t = 0; t < trips; ++t, row += p.stride, dr += step_d) {
-    const bool on = row < a.rows;
-    now_x = next_x;
-    now_g = next_g;
-    pos = next_pos;
-    xr += step_x;
-    gr += step_g;
-    if (row + p.stride < a.rows) {
-      next_g.load(gr, l);
-      if (norm) next_x.load(xr, l);
-      if (turns) next_pos = where.next(a, row + p.stride);
-    }
-    if (turns && on && (pos < 0 || pos >= a.table_rows)) {
-      atomicOr(a.status, kStatusBadShape);
-      pos = -1;
-    }
-    float xa[U][V], xb[U][V], za[U][V], zb[U][V], ss[2] = {0.f, 0.f}, gx[2] = {0.f, 0.f};
-    if (on && norm) {
-      now_x.get(xa, xb, l);
-      now_g.get(za, zb, l);
+  {
+    const Ring<T, V, U> ring{shared};
+    int row = p.row, ahead = row;  // the row that is fetched next
+    auto fetch = [&](int stage) {
+      if (ahead < a.rows) {
+        ring.fetch(stage, 0, gr, l);
+        ring.fetch(stage, 2 * U, xr, l);
+      }
+      copy_commit();
+      ahead += p.stride;
+      gr += step_g;
+      xr += step_x;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(i);
+    int stage = 0;
+    long long next_pos = a.rot > 0 && row < a.rows ? where.next(a, row) : -1;
+    const int trips = (a.rows + p.stride - 1) / p.stride;
+    for (int t = 0; t < trips; ++t, row += p.stride, dr += step_d) {
+      const bool on = row < a.rows;
+      fetch(stage == 0 ? kStages - 1 : stage - 1);
+      const long long pos = on && a.rot > 0 ? checked(a, next_pos) : -1;
+      if (a.rot > 0 && row + p.stride < a.rows) next_pos = where.next(a, row + p.stride);
+      float c[U][V], s[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (pos >= 0 && l.turn[u])
+          load_angles<V, NEIGHBOURS>(a.cos + pos * a.ldt, a.sin + pos * a.ldt, l.pair[u], l.second[u], c[u], s[u]);
+      copy_wait<kStages - 1>();  // the row's own copies; each lane reads only what it fetched
+      Vectors<T, V, U> vx, vg;
+      if (on) {
+        ring.read(vg, stage, 0, l);
+        ring.read(vx, stage, 2 * U, l);
+      }
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      float xa[U][V], xb[U][V], za[U][V], zb[U][V], ss[2] = {0.f, 0.f}, gx[2] = {0.f, 0.f};
+      vx.get(xa, xb, l);
+      vg.get(za, zb, l);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (turns && pos >= 0 && l.turn[u]) {
-          float c[V], s[V];
-          load_angles<V, NEIGHBOURS>(a.cos + pos * a.ldt, a.sin + pos * a.ldt, l.pair[u], l.second[u], c, s);
-          rotate<V, NEIGHBOURS, -1>(za[u], zb[u], c, s);
-        }
+        if (pos >= 0 && l.turn[u]) rotate<V, NEIGHBOURS, -1>(za[u], zb[u], c[u], s[u]);
         dot<V>(ss, xa[u], xa[u]);
         dot<V>(ss, xb[u], xb[u]);
-        float t_[V];
-        mul<V>(t_, xa[u], l.wa[u]);
-        dot<V>(gx, za[u], t_);
-        mul<V>(t_, xb[u], l.wb[u]);
-        dot<V>(gx, zb[u], t_);
+        float w_[V];
+        mul<V>(w_, xa[u], l.wa[u]);
+        dot<V>(gx, za[u], w_);
+        mul<V>(w_, xb[u], l.wb[u]);
+        dot<V>(gx, zb[u], w_);
       }
-    }
-    const float r = rsqrtf(group_sum<FULL>(ss[0] + ss[1], a, p.lane) * a.inv_dim + a.eps);
-    const float mean = group_sum<FULL>(gx[0] + gx[1], a, p.lane) * a.inv_dim * r * r;  // mean(g x r) r
-    if (!on) continue;
-    if (norm) {
+      const float r = rsqrtf(group_sum<FULL>(on ? ss[0] + ss[1] : 0.f, a, p) * a.inv_dim + a.eps);
+      const float mean = group_sum<FULL>(on ? gx[0] + gx[1] : 0.f, a, p) * a.inv_dim * r * r;  // mean(g x r) r
+      if (!on) continue;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float t_[V];
+        float w_[V];
         // dw += dz (x r);  dx = r (dz w - x mean)
-        mul<V>(t_, za[u], xa[u]);
-        mad<V>(da[u], t_, r, da[u]);
-        mul<V>(t_, zb[u], xb[u]);
-        mad<V>(db[u], t_, r, db[u]);
+        mul<V>(w_, za[u], xa[u]);
+        mad<V>(da[u], w_, r, da[u]);
+        mul<V>(w_, zb[u], xb[u]);
+        mad<V>(db[u], w_, r, db[u]);
         mul<V>(za[u], za[u], l.wa[u]);
         mul<V>(zb[u], zb[u], l.wb[u]);
         mad<V>(za[u], xa[u], -mean, za[u]);
         mad<V>(zb[u], xb[u], -mean, zb[u]);
         scale<V>(za[u], r);
         scale<V>(zb[u], r);
-        now_g.a[u].set(za[u]);
-        now_g.b[u].set(zb[u]);
+        vg.a[u].set(za[u]);
+        vg.b[u].set(zb[u]);
       }
+      vg.store(dr, l);
     }
-    now_g.store(dr, l);
   }
+  copy_wait<0>();
+  if (a.copies) copy_values<T, V>(dy, a.ldy, dx, a.lddx, a);
   if (part == nullptr) return;
-  const int heads = a.groups * (kThreads / 32);  // of the block
+  __syncthreads();  // the rings give way to the sums
+  float* sums = reinterpret_cast<float*>(shared);
+  const int sets = a.groups * (kThreads / 32);  // of the block
   const int sub = (threadIdx.x & 31) / a.group;
   if (sub < a.groups) {
     float* mine = sums + ((threadIdx.x >> 5) * a.groups + sub) * a.dim;
@@ -476,16 +559,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
   }
   __syncthreads();
-  const unsigned slot0 = blockIdx.x * heads;
+  const unsigned slot0 = blockIdx.x * sets;
   for (int c = threadIdx.x; c < 2 * a.dim; c += kThreads) {
     const bool keys = c >= a.dim;
     const int column = keys ? c - a.dim : c;
     float v = 0.f;
-    int head = slot0 % a.all_heads;
-    for (int g = 0; g < heads; ++g) {
-      const bool use = keys ? head >= a.heads && head < a.heads + a.kv_heads : head < a.heads;
-      if (use) v += sums[g * a.dim + column];
-      if (++head == a.all_heads) head = 0;
+    int set = slot0 % a.sets;
+    for (int g = 0; g < sets; ++g) {
+      if ((set >= a.q_sets) == keys) v += sums[g * a.dim + column];
+      if (++set == a.sets) set = 0;
     }
     part[static_cast<long long>(blockIdx.x) * 2 * a.dim + c] = v;
   }
@@ -657,16 +739,19 @@ void finish(Problem& p, std::initializer_list<const torch::Tensor*> packed, cons
   a.status = status_device_ptr();
 }
 
-constexpr int kMaxSmem = 16 << 10;  // of the weight gradients: 8 warps x 2 x 8 x 32 columns at most
+// Shared memory of the backward kernels: the rings (48 KB at most).  The weight gradients' sums
+// that take their place need 8 warps x 2 V U x 32 columns at most, a third of that.
+template <typename T, int V, int U>
+constexpr int kBwdSmem = std::max(Ring<T, V, U>::kSize, kThreads / 32 * 64 * V * U * 4);
 
 // Blocks of a kernel that fit on an SM of the current device.
-template <auto Kernel>
+template <auto Kernel, int Smem>
 int resident(int device) {
   static std::atomic<int> known[64];
   std::atomic<int>& k = known[device & 63];
   int n = k.load(std::memory_order_relaxed);
   if (n == 0) {
-    REVPP_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, kThreads, kMaxSmem));
+    REVPP_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, kThreads, Smem));
     n = std::max(1, n);
     k.store(n, std::memory_order_relaxed);
   }
@@ -674,13 +759,19 @@ int resident(int device) {
 }
 
 // Blocks for one resident wave, or fewer when the rows need fewer.
-template <auto Kernel>
+template <auto Kernel, int Smem>
 int blocks_for(const QkArgs& a, int device) {
   const int per_block = a.groups * (kThreads / 32);
-  const long long need = (static_cast<long long>(a.rows) * a.all_heads + per_block - 1) / per_block;
-  const long long least = (a.all_heads + per_block - 1) / per_block;
-  const long long wave = static_cast<long long>(resident<Kernel>(device)) * num_sms();
+  const long long need = (static_cast<long long>(a.rows) * a.sets + per_block - 1) / per_block;
+  const long long least = (a.sets + per_block - 1) / per_block;
+  const long long wave = static_cast<long long>(resident<Kernel, Smem>(device)) * num_sms();
   return static_cast<int>(std::max(least, std::min(need, wave)));
+}
+
+// Sets of h query or key heads.
+void make_sets(QkArgs& a, int h) {
+  a.q_sets = (a.heads + h - 1) / h;
+  a.sets = a.q_sets + (a.kv_heads + h - 1) / h;
 }
 
 template <typename F>
@@ -722,12 +813,13 @@ void qk_norm_rope_fwd(const torch::Tensor& qkv, torch::Tensor out, int64_t heads
   finish(p, {&qkv, &out}, wq, wk, cos, sin, positions, S, interleaved);
   QkArgs& a = p.a;
   a.ldy = out.stride(0);
-  a.all_heads = a.heads + a.kv_heads * (qkv.data_ptr() == out.data_ptr() ? 1 : 2);
+  make_sets(a, kFwdHeads);
+  a.copies = qkv.data_ptr() != out.data_ptr();
   by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb, auto full) {
     using T = decltype(e);
     constexpr auto kernel =
-        &qk_norm_rope_fwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value, decltype(full)::value>;
-    launch_pdl(kernel, dim3(blocks_for<kernel>(a, qkv.get_device())), dim3(kThreads), 0, cur_stream(),
+        &qk_norm_rope_fwd_kernel<T, decltype(v)::value, decltype(u)::value, kFwdHeads, decltype(nb)::value, decltype(full)::value>;
+    launch_pdl(kernel, dim3(blocks_for<kernel, 0>(a, qkv.get_device())), dim3(kThreads), 0, cur_stream(),
                static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(out.data_ptr()), a);
   });
   REVPP_CHECK_LAUNCH();
@@ -765,14 +857,14 @@ void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch
     finish(p, {&qkv, &dout, &dqkv}, wq, wk, cos, sin, positions, S, interleaved);
     a.ldy = dout.stride(0);
     a.lddx = dqkv.stride(0);
-    a.all_heads = a.heads + a.kv_heads * (dout.data_ptr() == dqkv.data_ptr() ? 1 : 2);
-    const size_t smem = weights ? static_cast<size_t>(kThreads / 32) * a.groups * a.dim * 4 : 0;
-    REVPP_CHECK(smem <= kMaxSmem, "shared memory");
+    make_sets(a, 1);
+    a.copies = dout.data_ptr() != dqkv.data_ptr();
     by_type(p, qkv.scalar_type(), interleaved, [&](auto e, auto v, auto u, auto nb, auto full) {
       using T = decltype(e);
       constexpr auto kernel =
           &qk_norm_rope_bwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value, decltype(full)::value>;
-      blocks = blocks_for<kernel>(a, qkv.get_device());
+      constexpr int smem = kBwdSmem<T, decltype(v)::value, decltype(u)::value>;
+      blocks = blocks_for<kernel, smem>(a, qkv.get_device());
       if (weights) part = torch::empty({static_cast<int64_t>(blocks) * 2 * a.dim}, qkv.options().dtype(at::kFloat));
       launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, cur_stream(), static_cast<const T*>(dout.data_ptr()),
                  static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(dqkv.data_ptr()), a,
