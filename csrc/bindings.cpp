@@ -98,8 +98,7 @@ void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch
                       const c10::optional<torch::Tensor>& positions, const c10::optional<int64_t>& S, bool interleaved,
                       bool accumulate);
 // grad_clip.cu
-torch::Tensor clip_grads(const std::vector<torch::Tensor>& grads, double max_norm,
-                         const c10::optional<std::vector<torch::Tensor>>& out, bool max_type);
+torch::Tensor clip_grads(const py::list& grads, double max_norm, const c10::optional<py::list>& out, bool max_type);
 // host.cpp
 void set_sm_reserve(int n);
 int sm_reserve();

@@ -10,11 +10,12 @@
 // arrive; here the tokens are sorted by id (stable, so each row's terms come in token order)
 // and every dW row is written once, so equal inputs give equal bits.
 //
-//  1. embed_sort_kernel: 2^c CTAs, each owns the ids with its own low c bits (frequent tokens,
-//     which vocabularies number low, spread over the CTAs), reads all n ids, counts those of the
-//     CTAs before it (its offset in the sorted order, with no exchange between CTAs) and places
-//     its own by a counting sort.  Warp w reads the w-th part of the tokens and keeps its own
-//     counters, so that the order within an id is the token order.
+//  1. embed_sort_kernel: 2^c bins, each of the ids with the same low c bits (frequent tokens, which
+//     vocabularies number low, spread over the bins).  A cluster of four CTAs per bin reads all n ids,
+//     a quarter each, counts those of earlier bins (the bin's offset in the sorted order, with no
+//     exchange between clusters) and places its own by a counting sort: the CTAs' counts meet over
+//     distributed shared memory, and within a CTA up to 16 warps take consecutive parts of its tokens,
+//     so that the order within an id is the token order.
 //  2. embed_reduce_kernel: one CTA per (chunk of sorted tokens, slab of columns).  Each warp adds
 //     the rows of its part of the chunk run by run in registers and writes the runs that lie
 //     inside; runs that cross warps meet in shared memory, and runs that cross chunks leave one
@@ -24,11 +25,15 @@
 #include <algorithm>
 #include <atomic>
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "host.h"
 #include "vec.cuh"
 
 namespace revpp {
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -36,8 +41,10 @@ constexpr int kThreads = 256;
 constexpr int kFwdUnroll = 4;      // vectors per lane and row slab
 constexpr int kSortWarps = 32;
 constexpr int kSortPer = 1024;     // tokens a warp lists at most before they are placed
-constexpr int kSortLogCtas = 7;    // at most one CTA per SM, unless the table is very long
-constexpr int kSortLogRange = 9;   // ids per CTA: 512 at most
+constexpr int kSortCluster = 4;    // CTAs that share a bin of ids, each with a part of the tokens
+constexpr int kSortLogBins = 5;    // at most one CTA per SM, unless the table is very long
+constexpr int kSortLogRange = 10;  // ids per bin: 1024 at most, one per thread
+constexpr int kRankers = 16;       // warps that place tokens
 constexpr int kWarps = 4;          // of a reduce CTA
 constexpr int kWarpTokens = 8;    // sorted tokens a reduce warp adds: all their rows are in flight at once
 constexpr int kChunk = kWarps * kWarpTokens;
@@ -65,28 +72,41 @@ __global__ void __launch_bounds__(kThreads)
   const TW* src = w + (ok ? id : 0) * ldw;
   TO* dst = out + row * ldo;
   const int c0 = ((slab * kFwdUnroll << log_l) + sub) * V;
-  Pack<TW, V> x[kFwdUnroll];
+  constexpr int P = V * sizeof(TW) <= 16 ? V : 16 / sizeof(TW), Q = V * sizeof(TO) <= 16 ? V : 16 / sizeof(TO);
+  Pack<TW, P> x[kFwdUnroll][V / P];
 #pragma unroll
   for (int u = 0; u < kFwdUnroll; ++u) {
     const int c = c0 + ((u * V) << log_l);
-    if (c < H && ok) x[u] = Pack<TW, V>::load_ro(src + c);
+#pragma unroll
+    for (int i = 0; i < V / P; ++i)
+      if (c < H && ok) x[u][i] = Pack<TW, P>::load_ro(src + c + i * P);
   }
 #pragma unroll
   for (int u = 0; u < kFwdUnroll; ++u) {
     const int c = c0 + ((u * V) << log_l);
     if (c >= H) continue;
     float f[V];
-    x[u].get(f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = ok ? f[j] * scale : 0.f;
-    Pack<TO, V> y;
-    y.set(f);
-    y.store(dst + c);
+    for (int i = 0; i < V / P; ++i) {
+      float g[P];
+      x[u][i].get(g);
+#pragma unroll
+      for (int j = 0; j < P; ++j) f[i * P + j] = ok ? g[j] * scale : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < V / Q; ++i) {
+      float g[Q];
+#pragma unroll
+      for (int j = 0; j < Q; ++j) g[j] = f[i * Q + j];
+      Pack<TO, Q> y;
+      y.set(g);
+      y.store(dst + c + i * Q);
+    }
   }
 }
 
 // ------------------------------------------------------------------ backward: sort
-// An id's place in the sorted order follows from its slot: the CTA that sorts it, then the rest.
+// An id's place in the sorted order follows from its slot: its bin, then the rest.
 struct EmbedWs {
   int* start;     // [slots + 1] first sorted position of each slot
   int* order;     // [n] token of each sorted position
@@ -108,12 +128,12 @@ __device__ __forceinline__ unsigned checked(int32_t id, unsigned vocab) {
   return lo < vocab ? lo : 0xffffffffu;
 }
 
-// The tokens [beg, end) of one warp whose slots belong to CTA `cta` go to `list` in token order, as
-// (token - seg) << 9 | local id, and are counted per local id; returns how many.  `less` counts the
-// ids of earlier CTAs.  A lane reads two neighbouring ids per access (`wide`: the address allows it).
+// The tokens [beg, end) of one warp whose ids belong to `bin` go to `list` in token order, as
+// (token - seg) << kSortLogRange | local id, and are counted per local id; returns how many.  `less`
+// counts the ids of earlier bins.  A lane reads two neighbouring ids per access (`wide`: the address allows it).
 template <typename TI>
 __device__ __forceinline__ int sweep(const TI* __restrict__ ids, int seg, int beg, int end, bool wide, unsigned vocab,
-                                     unsigned padding, unsigned cta, int log_c, int lane, int* list, int* count, int& less,
+                                     unsigned padding, unsigned bin, int log_c, int lane, int* list, int* count, int& less,
                                      bool& bad) {
   constexpr int kPairs = 8;
   const unsigned low = (1u << log_c) - 1, before = (1u << lane) - 1;
@@ -128,7 +148,7 @@ __device__ __forceinline__ int sweep(const TI* __restrict__ ids, int seg, int be
         const Raw raw = __ldg(reinterpret_cast<const Raw*>(ids + t));
         id[u][0] = checked(reinterpret_cast<const TI*>(&raw)[0], vocab);
         id[u][1] = checked(reinterpret_cast<const TI*>(&raw)[1], vocab);
-        if (cta == 0) bad |= id[u][0] == 0xffffffffu || id[u][1] == 0xffffffffu;
+        if (bin == 0) bad |= id[u][0] == 0xffffffffu || id[u][1] == 0xffffffffu;
       } else {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -148,8 +168,8 @@ __device__ __forceinline__ int sweep(const TI* __restrict__ ids, int seg, int be
       for (int e = 0; e < 2; ++e) {
         const unsigned k = id[u][e];
         const unsigned c = k == padding || k == 0xffffffffu ? 0xffffffffu : k & low;
-        less += c < cta;
-        in[e] = c == cta;
+        less += c < bin;
+        in[e] = c == bin;
       }
       if (!__any_sync(0xffffffffu, in[0] || in[1])) continue;
       const unsigned m0 = __ballot_sync(0xffffffffu, in[0]), m1 = __ballot_sync(0xffffffffu, in[1]);
@@ -160,7 +180,7 @@ __device__ __forceinline__ int sweep(const TI* __restrict__ ids, int seg, int be
         if (in[e]) {
           const int local = static_cast<int>(id[u][e] >> log_c);
           list[at++] = (t + e) << kSortLogRange | local;
-          if (count != nullptr) atomicAdd(count + local, 1);
+          atomicAdd(count + local, 1);
         }
       len += __popc(m0) + __popc(m1);
     }
@@ -178,69 +198,96 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 }
 
 template <typename TI>
-__global__ void __launch_bounds__(kSortWarps * 32, 1)
+__global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarps * 32, 1)
     embed_sort_kernel(const TI* __restrict__ ids, int n, int per, unsigned vocab, unsigned padding, EmbedWs ws,
                       int* __restrict__ status) {
-  // [kSortWarps][per] tokens of each warp, [kSortWarps][range] offsets of each ranking warp
+  // [kSortWarps][per] tokens of each warp, [kRankers][range] next positions of each ranking warp
   extern __shared__ int sm[];
-  __shared__ int s_count[1 << kSortLogRange];  // tokens of each local id, then its next position
+  __shared__ int s_count[1 << kSortLogRange];  // tokens of each local id: of all segments, then of one
+  __shared__ int s_next[1 << kSortLogRange];   // position of the next token of each local id
   __shared__ int s_less[kSortWarps], s_len[kSortWarps], s_sum[kSortWarps], s_off[kSortWarps];
+  cg::cluster_group cluster = cg::this_cluster();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int range = 1 << ws.log_r;
-  const int cta = blockIdx.x;
-  const int segment = kSortWarps * per;  // tokens whose lists fit into shared memory
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int bin = blockIdx.x / kSortCluster;
+  const int share = kSortWarps * per;           // tokens of a CTA whose lists fit into shared memory
+  const int segment = kSortCluster * share;
+  const int slot = threadIdx.x;                 // the thread's local id, where slot < range
   int* list = sm + warp * per;
   int* hist = sm + kSortWarps * per;
-  if (threadIdx.x < range) s_count[threadIdx.x] = 0;
+  s_count[slot] = 0;
   __syncthreads();
   pdl_wait();
   pdl_trigger();
   const bool wide = reinterpret_cast<uintptr_t>(ids) % (2 * sizeof(TI)) == 0;
   int len = 0, less = 0;
   bool bad = false;
-  for (int seg = 0; seg < n; seg += segment) {
-    const int beg = min(n, seg + warp * per);
-    len = sweep(ids, seg, beg, min(n, beg + per), wide, vocab, padding, cta, ws.log_c, lane, list, s_count, less, bad);
-  }
-  if (blockIdx.x == 0 && bad) atomicOr(status, kStatusBadShape);
+  auto take = [&](int seg) {  // this warp's part of a segment
+    const long long from = static_cast<long long>(seg) + rank * share + warp * per;
+    const int beg = static_cast<int>(min(from, static_cast<long long>(n)));
+    const int end = static_cast<int>(min(from + per, static_cast<long long>(n)));
+    len = sweep(ids, seg, beg, end, wide, vocab, padding, bin, ws.log_c, lane, list, s_count, less, bad);
+  };
+  // sum of every CTA's count of the thread's local id, and of the CTAs before this one
+  auto gather = [&](int& earlier) {
+    int total = 0;
+    earlier = 0;
+#pragma unroll
+    for (int r = 0; r < kSortCluster; ++r) {
+      const int c = cluster.map_shared_rank(s_count, r)[slot];
+      total += c;
+      earlier += r < rank ? c : 0;
+    }
+    return total;
+  };
+  for (long long seg = 0; seg < n; seg += segment) take(static_cast<int>(seg));
+  if (bin == 0 && bad) atomicOr(status, kStatusBadShape);
   less = warp_sum(less);
-  if (lane == 0) {
-    s_less[warp] = less;
-    s_len[warp] = len;
-  }
-  __syncthreads();
-  // first position of each local id: the tokens of earlier CTAs, and of smaller local ids
-  const int total = threadIdx.x < range ? s_count[threadIdx.x] : 0;
+  if (lane == 0) s_less[warp] = less;
+  cluster.sync();
+  // first position of each local id: the tokens of earlier bins, and of smaller local ids
+  int earlier;
+  const int total = gather(earlier);
+  int base = 0;
+#pragma unroll
+  for (int r = 0; r < kSortCluster; ++r) base += cluster.map_shared_rank(s_less, r)[lane];
+  base = warp_sum(base);
   const int incl = warp_scan(total, lane);
   if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  const int base = warp_sum(s_less[lane]);
-  if (threadIdx.x < range) {
-    int first = base + incl - total;
-    for (int w = 0; w < warp; ++w) first += s_sum[w];
-    s_count[threadIdx.x] = first;
-    ws.start[cta * range + threadIdx.x] = first;
-    if (cta == gridDim.x - 1 && threadIdx.x == range - 1) ws.start[ws.slots()] = first + total;
+  const int first = base + warp_sum(lane < warp ? s_sum[lane] : 0) + incl - total;
+  const bool many = n > segment;
+  s_next[slot] = first + (many ? 0 : earlier);
+  if (rank == 0 && slot < range) {
+    ws.start[bin * range + slot] = first;
+    if (blockIdx.x + kSortCluster >= gridDim.x && slot == range - 1) ws.start[ws.slots()] = first + total;
   }
-  for (int seg = 0; seg < n; seg += segment) {
-    if (n > segment) {  // the lists hold the last segment only
+  for (long long seg = 0; seg < n; seg += segment) {
+    int of_segment = 0;
+    if (many) {  // the lists hold the last segment only
+      cluster.sync();  // all have read the counts
+      s_count[slot] = 0;
       __syncthreads();
-      const int beg = min(n, seg + warp * per);
-      len = sweep(ids, seg, beg, min(n, beg + per), wide, vocab, padding, cta, ws.log_c, lane, list, static_cast<int*>(nullptr),
-                  less, bad);
-      if (lane == 0) s_len[warp] = len;
-      __syncthreads();
+      take(static_cast<int>(seg));
+      cluster.sync();
+      of_segment = gather(earlier);
+      of_segment -= earlier;  // of this CTA and those behind it
+      s_next[slot] += earlier;
     }
-    // `rankers` warps share the segment's tokens, 64 or more each, in token order
+    if (lane == 0) s_len[warp] = len;
+    __syncthreads();
+    // `rankers` warps share the CTA's tokens, 64 or more each, in token order
     const int mine = s_len[lane];
     const int ends = warp_scan(mine, lane);
     const int m = __shfl_sync(0xffffffffu, ends, 31);
-    const int rankers = max(1, min(kSortWarps, (m + 63) / 64));
-    const int share = ((m + rankers - 1) / rankers + 31) & ~31;
+    const int rankers = max(1, min(kRankers, (m + 63) / 64));
+    const int each = ((m + rankers - 1) / rankers + 31) & ~31;
     if (warp == 0) s_off[lane] = ends - mine;
-    for (int i = threadIdx.x; i < rankers * range; i += kSortWarps * 32) hist[i] = 0;
+    if (rankers > 1)
+      for (int i = threadIdx.x; i < rankers * range; i += kSortWarps * 32) hist[i] = 0;
     __syncthreads();
-    // item i of the segment lies in the last list that starts at or before i
+    // item i lies in the last list that starts at or before i
     auto item_at = [&](int i) {
       int w = 0;
 #pragma unroll
@@ -248,42 +295,46 @@ __global__ void __launch_bounds__(kSortWarps * 32, 1)
         if (s_off[w + o] <= i) w += o;
       return sm[w * per + i - s_off[w]];
     };
-    const int i0 = warp * share, i1 = min(m, i0 + share);
-    int* my = hist + warp * range;
+    const int i0 = min(m, warp * each), i1 = min(m, i0 + each);
+    int* my = s_next;
     constexpr int kLocal = (1 << kSortLogRange) - 1;
     if (rankers > 1) {
+      my = hist + min(warp, kRankers - 1) * range;  // the warps behind the rankers have no tokens
       for (int i = i0 + lane; i < i1; i += 32) atomicAdd(my + (item_at(i) & kLocal), 1);
       __syncthreads();
-    }
-    if (threadIdx.x < range) {
-      int at = s_count[threadIdx.x];
-      if (rankers > 1) {
+      if (slot < range) {
+        int at = s_next[slot];
         for (int w = 0; w < rankers; ++w) {
-          const int c = hist[w * range + threadIdx.x];
-          hist[w * range + threadIdx.x] = at;
+          const int c = hist[w * range + slot];
+          hist[w * range + slot] = at;
           at += c;
         }
-        s_count[threadIdx.x] = at;
+        s_next[slot] = at;
       }
+      __syncthreads();
     }
-    if (rankers > 1) __syncthreads();
-    else my = s_count;
     for (int i = i0; i < i1; i += 32) {
       const bool on = i + lane < i1;
       const int item = on ? item_at(i + lane) : 0;
       const int k = on ? item & kLocal : -1;
       const unsigned same = __match_any_sync(0xffffffffu, k);
-      const int rank = __popc(same & ((1u << lane) - 1));
+      const int before = __popc(same & ((1u << lane) - 1));
       if (on) {
-        const int at = my[k] + rank;
-        ws.order[at] = seg + (static_cast<unsigned>(item) >> kSortLogRange);
-        ws.key[at] = cta * range + k;
+        const int at = my[k] + before;
+        ws.order[at] = static_cast<int>(seg) + (static_cast<unsigned>(item) >> kSortLogRange);
+        ws.key[at] = bin * range + k;
       }
       __syncwarp();
-      if (on && rank == 0) my[k] += __popc(same);
+      if (on && before == 0) my[k] += __popc(same);
       __syncwarp();
     }
+    if (many) {
+      // s_next stands behind this CTA's tokens: the next segment begins behind those of the others too
+      __syncthreads();
+      s_next[slot] += of_segment - s_count[slot];
+    }
   }
+  cluster.sync();  // the others may still read this CTA's counts
 }
 
 // ------------------------------------------------------------------ backward: reduce
@@ -550,7 +601,7 @@ Plan plan_bwd(long long n, long long vocab, int H, int v) {
   p.v = v;
   p.slabs = (H + kSlab - 1) / kSlab;
   p.log_c = 0;
-  while (p.log_c < kSortLogCtas && (1LL << p.log_c) < vocab) ++p.log_c;
+  while (p.log_c < kSortLogBins && (1LL << p.log_c) < vocab) ++p.log_c;
   p.log_r = 0;
   while ((1LL << (p.log_c + p.log_r)) < vocab) ++(p.log_r < kSortLogRange ? p.log_r : p.log_c);
   p.chunks = (n + kChunk - 1) / kChunk;
@@ -578,9 +629,12 @@ void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tens
   check_same_device(w, out, "w and out");
   c10::cuda::CUDAGuard guard(w.device());
   const int H = static_cast<int>(w.size(1));
-  const int top = 16 / static_cast<int>(std::max(w.element_size(), out.element_size()));
-  int v = top;
-  while (v > 1 && !(H % v == 0 && rows_allow(w, w.stride(0), vocab, v) && rows_allow(out, out.stride(0), n, v))) v /= 2;
+  // the narrower type in 16-byte accesses, the other in one or two
+  const int w_most = 16 / static_cast<int>(w.element_size()), out_most = 16 / static_cast<int>(out.element_size());
+  int v = std::max(w_most, out_most);
+  while (v > 1 && !(H % v == 0 && rows_allow(w, w.stride(0), vocab, std::min(v, w_most)) &&
+                    rows_allow(out, out.stride(0), n, std::min(v, out_most))))
+    v /= 2;
   int log_l = 0;
   while (log_l < 5 && (1 << log_l) * v < H) ++log_l;
   const int per_slab = (kFwdUnroll << log_l) * v;
@@ -596,7 +650,7 @@ void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tens
       auto go = [&](auto ti, auto vc) {
         using TI = decltype(ti);
         constexpr int V = decltype(vc)::value;
-        if constexpr (V * std::max(sizeof(TW), sizeof(TO)) <= 16)
+        if constexpr (V * std::min(sizeof(TW), sizeof(TO)) <= 16)
           launch_pdl(embed_fwd_kernel<TI, TW, TO, V>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, cur_stream(),
                      static_cast<const TI*>(ids.data_ptr()), static_cast<const TW*>(w.data_ptr()),
                      static_cast<long long>(w.stride(0)), static_cast<TO*>(out.data_ptr()),
@@ -641,9 +695,10 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
   EmbedWs ws{reinterpret_cast<int*>(base), reinterpret_cast<int*>(base + p.off_order),
              reinterpret_cast<int*>(base + p.off_key), reinterpret_cast<float*>(base + p.off_part), p.log_c, p.log_r};
   int* status = status_device_ptr();
-  // every warp lists a 32nd of the tokens, in segments of 32 x kSortPer where there are more
-  const int per = static_cast<int>(std::min<long long>(kSortPer, (n + kSortWarps * 64 - 1) / (kSortWarps * 64) * 64));
-  const size_t smem = static_cast<size_t>(kSortWarps) * ((1 << p.log_r) + per) * 4;
+  // the cluster's warps list all tokens, in segments where there are more than kSortPer for each
+  constexpr int kLists = kSortCluster * kSortWarps;
+  const int per = static_cast<int>(std::min<long long>(kSortPer, (n + kLists * 64 - 1) / (kLists * 64) * 64));
+  const size_t smem = (static_cast<size_t>(kRankers << p.log_r) + kSortWarps * per) * 4;
   const unsigned padding = padding_idx >= 0 && padding_idx < vocab ? static_cast<unsigned>(padding_idx) : 0xffffffffu;
   auto sort = [&](auto ti) {
     using TI = decltype(ti);
@@ -651,10 +706,10 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
     const uint64_t bit = 1ull << (dw.get_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
       REVPP_CUDA_CHECK(cudaFuncSetAttribute(embed_sort_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            kSortWarps * ((1 << kSortLogRange) + kSortPer) * 4));
+                                            ((kRankers << kSortLogRange) + kSortWarps * kSortPer) * 4));
       ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    launch_pdl(embed_sort_kernel<TI>, dim3(1u << p.log_c), dim3(kSortWarps * 32), smem, cur_stream(),
+    launch_pdl(embed_sort_kernel<TI>, dim3(kSortCluster << p.log_c), dim3(kSortWarps * 32), smem, cur_stream(),
                static_cast<const TI*>(ids.data_ptr()), static_cast<int>(n), per, static_cast<unsigned>(vocab), padding, ws, status);
   };
   if (ids.scalar_type() == at::kLong) sort(int64_t{});

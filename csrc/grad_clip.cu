@@ -6,7 +6,7 @@
 //
 // Two launches for any number of tensors up to the table's size: the first reads every gradient
 // and leaves one partial per block, the second adds the partials (each block by itself, in a fixed
-// order) and scales.  The table of tensors travels in the kernel's parameters, so a captured graph
+// order) and scales, from the last chunk to the first: what was read last is still in L2.  The table of tensors travels in the kernel's parameters, so a captured graph
 // keeps it and nothing is copied to the device.  Squares are summed in 64 bits: gradients from 1e-30
 // to 1e30 neither vanish nor overflow, and the result does not depend on how tensors are cut.
 // A NaN makes the norm and every output NaN, an infinity makes finite outputs 0, as in the formula.
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(norm);
   const double ratio = max_norm / (norm + 1e-6);
   const float coef = ratio > 1.0 ? 1.f : static_cast<float>(ratio);  // a NaN stays
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  for (int c = t.chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
     const Entry& e = t.e[entry_of(t, c)];
     if (coef == 1.f && e.dst == e.src) continue;
     if (e.src_type == kF32) scale_to<float>(e, c, coef);
@@ -234,32 +234,38 @@ bool same_layout(const torch::Tensor& a, const torch::Tensor& b) {
 
 struct Range {
   uintptr_t lo, hi;
-  int64_t index;
-  bool written;
+  int index;
 };
 
 // No output may share memory with another output or with another tensor's gradient.
-void check_overlaps(const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>& outs) {
-  std::vector<Range> r;
-  r.reserve(grads.size() * 2);
-  for (size_t i = 0; i < grads.size(); ++i) {
-    if (grads[i].numel() == 0) continue;
-    const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i].data_ptr()), o = reinterpret_cast<uintptr_t>(outs[i].data_ptr());
-    const bool same = g == o && grads[i].scalar_type() == outs[i].scalar_type();
-    r.push_back({o, o + outs[i].nbytes(), static_cast<int64_t>(i), true});
-    if (!same) r.push_back({g, g + grads[i].nbytes(), static_cast<int64_t>(i), false});
+void check_overlaps(const std::vector<Entry>& es, const std::vector<int>& indexes) {
+  auto size = [](int type) { return type == kF32 ? 4 : 2; };
+  std::vector<Range> outs(es.size());
+  uintptr_t grads_lo = ~uintptr_t(0), grads_hi = 0;  // of the gradients that are not their own outputs
+  for (size_t i = 0; i < es.size(); ++i) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(es[i].dst), g = reinterpret_cast<uintptr_t>(es[i].src);
+    outs[i] = {o, o + es[i].n * size(es[i].dst_type), static_cast<int>(i)};
+    if (o != g || es[i].dst_type != es[i].src_type) {
+      grads_lo = std::min(grads_lo, g);
+      grads_hi = std::max<uintptr_t>(grads_hi, g + es[i].n * size(es[i].src_type));
+    }
   }
   auto before = [](const Range& a, const Range& b) { return a.lo < b.lo; };
-  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
-  // the furthest end among all ranges so far, and among the written ones
-  uintptr_t any = 0, written = 0;
-  int64_t any_i = -1, written_i = -1;
-  for (const Range& x : r) {
-    const bool clash = x.written ? x.lo < any : x.lo < written;
-    REVPP_CHECK(!clash, "out ", x.written ? x.index : written_i, " shares memory with the tensors at ",
-                x.written ? any_i : x.index, ": outputs must be distinct, or their own gradients");
-    if (x.hi > any) any = x.hi, any_i = x.index;
-    if (x.written && x.hi > written) written = x.hi, written_i = x.index;
+  if (!std::is_sorted(outs.begin(), outs.end(), before)) std::sort(outs.begin(), outs.end(), before);
+  for (size_t i = 1; i < outs.size(); ++i)
+    REVPP_CHECK(outs[i].lo >= outs[i - 1].hi, "out ", indexes[outs[i].index], " shares memory with out ",
+                indexes[outs[i - 1].index], ": outputs must be distinct");
+  if (grads_lo >= outs.back().hi || grads_hi <= outs.front().lo) return;
+  for (size_t i = 0; i < es.size(); ++i) {
+    const uintptr_t g = reinterpret_cast<uintptr_t>(es[i].src), end = g + es[i].n * size(es[i].src_type);
+    // the last output that starts before the gradient's end
+    auto it = std::lower_bound(outs.begin(), outs.end(), end, [](const Range& r, uintptr_t v) { return r.lo < v; });
+    for (; it != outs.begin() && (it - 1)->hi > g; --it) {
+      const Range& r = *(it - 1);
+      const bool own = r.index == static_cast<int>(i) && r.lo == g && es[i].dst_type == es[i].src_type;
+      REVPP_CHECK(own, "out ", indexes[r.index], " shares memory with gradient ", indexes[i],
+                  ": an output must be its own gradient, or lie apart from all of them");
+    }
   }
 }
 
@@ -303,40 +309,52 @@ void run_clip(const std::vector<Entry>& es, double max_norm, const torch::Tensor
 
 }  // namespace
 
-torch::Tensor clip_grads(const std::vector<torch::Tensor>& grads, double max_norm,
-                         const c10::optional<std::vector<torch::Tensor>>& out, bool max_type) {
-  REVPP_CHECK(!grads.empty(), "grads must not be empty");
+// `grads` and `out` are Python lists (taken as they are: a list of hundreds of tensors is called once
+// per training step, and converting it would cost more than the checks).
+torch::Tensor clip_grads(const py::list& grads, double max_norm, const c10::optional<py::list>& out, bool max_type) {
+  const Py_ssize_t n = PyList_GET_SIZE(grads.ptr());
+  REVPP_CHECK(n > 0, "grads must not be empty");
   REVPP_CHECK(max_norm >= 0.0, "max_norm must not be negative or NaN");
-  const std::vector<torch::Tensor>& outs = out.has_value() ? *out : grads;
-  REVPP_CHECK(outs.size() == grads.size(), "out must have one tensor per gradient: ", outs.size(), " for ", grads.size());
-  std::vector<Entry> es;
-  es.reserve(grads.size());
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const torch::Tensor &g = grads[i], &o = outs[i];
-    const int gt = type_of(g), ot = type_of(o);
-    REVPP_CHECK(gt >= 0 && ot >= 0, "tensor ", i, " must be float32, bfloat16 or float16");
+  PyObject* outs = out.has_value() ? out->ptr() : grads.ptr();
+  REVPP_CHECK(PyList_GET_SIZE(outs) == n, "out must have one tensor per gradient: ", PyList_GET_SIZE(outs), " for ", n);
+  auto tensor = [](PyObject* list, Py_ssize_t i, const char* name) -> const torch::Tensor& {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    REVPP_CHECK(THPVariable_Check(o), name, " ", i, " is not a tensor");
+    return THPVariable_Unpack(o);
+  };
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const torch::Tensor &g = tensor(grads.ptr(), i, "gradient"), &o = tensor(outs, i, "out");
+    REVPP_CHECK(type_of(g) >= 0 && type_of(o) >= 0, "tensor ", i, " must be float32, bfloat16 or float16");
     REVPP_CHECK(g.layout() == at::kStrided && o.layout() == at::kStrided, "tensor ", i, " must be dense");
-    REVPP_CHECK(g.is_non_overlapping_and_dense(), "gradient ", i, " has gaps or repeats in memory: make it contiguous");
+    REVPP_CHECK(g.is_contiguous() || g.is_non_overlapping_and_dense(), "gradient ", i,
+                " has gaps or repeats in memory: make it contiguous");
     REVPP_CHECK(same_layout(g, o), "out ", i, " must have its gradient's sizes and strides");
   }
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const torch::Tensor &g = grads[i], &o = outs[i];
+  std::vector<Entry> es;
+  std::vector<int> indexes;
+  es.reserve(n);
+  indexes.reserve(n);
+  const torch::Tensor& front = tensor(grads.ptr(), 0, "gradient");
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const torch::Tensor &g = tensor(grads.ptr(), i, "gradient"), &o = tensor(outs, i, "out");
     REVPP_CHECK(g.is_cuda(), "gradient ", i, " must be a CUDA tensor");
-    REVPP_CHECK(g.device() == grads[0].device() && o.device() == g.device(), "all tensors must be on one device");
+    REVPP_CHECK(g.device() == front.device() && o.device() == g.device(), "all tensors must be on one device");
     if (g.numel() == 0) continue;
-    const int gt = type_of(g), ot = type_of(o);
-    const bool wide = reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0;
-    es.push_back({g.data_ptr(), o.data_ptr(), g.numel(), 0, static_cast<unsigned char>(gt), static_cast<unsigned char>(ot),
+    const void* src = g.data_ptr();
+    void* dst = o.data_ptr();
+    const bool wide = (reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) % 16 == 0;
+    es.push_back({src, dst, g.numel(), 0, static_cast<unsigned char>(type_of(g)), static_cast<unsigned char>(type_of(o)),
                   static_cast<unsigned char>(wide), 0});
+    indexes.push_back(static_cast<int>(i));
   }
-  check_overlaps(grads, outs);
-  c10::cuda::CUDAGuard guard(grads[0].device());
-  torch::Tensor norm = torch::empty({}, grads[0].options().dtype(at::kFloat));
+  c10::cuda::CUDAGuard guard(front.device());
+  torch::Tensor norm = torch::empty({}, front.options().dtype(at::kFloat));
   if (es.empty()) return norm.zero_();
+  check_overlaps(es, indexes);
   auto go = [&](auto cap) {
     constexpr int CAP = decltype(cap)::value;
-    if (max_type) run_clip<CAP, true>(es, max_norm, norm, grads[0].options());
-    else run_clip<CAP, false>(es, max_norm, norm, grads[0].options());
+    if (max_type) run_clip<CAP, true>(es, max_norm, norm, front.options());
+    else run_clip<CAP, false>(es, max_norm, norm, front.options());
   };
   if (es.size() <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 512>{});

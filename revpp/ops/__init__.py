@@ -181,7 +181,7 @@ def clip_grads(grads, max_norm: float, out=None, norm_type: float = 2.0) -> torc
     any gradient makes the norm and every output NaN."""
     if norm_type not in (2.0, float("inf")):
         raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
-    return ext().clip_grads(grads, max_norm, out, norm_type != 2.0)
+    return ext().clip_grads(list(grads), max_norm, None if out is None else list(out), norm_type != 2.0)
 
 
 __all__ = [
