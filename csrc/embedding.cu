@@ -507,51 +507,81 @@ __global__ void __launch_bounds__(kWarps * 32, 5)
   }
 }
 
-// Runs that cross chunks: the CTA of the chunk where one begins adds its pieces, one per chunk; warp w
-// takes every eighth, then the warps in turn.
+// Runs that cross chunks: a warp looks at one chunk's end and, where a run that began in the chunk
+// goes on, adds its pieces, one per chunk, in order.  The pieces of long runs (more than kOwnPieces)
+// are added by all of the CTA's warps: warp w takes every eighth, then the warps in turn.
+constexpr int kJoinWarps = kThreads / 32, kOwnPieces = 4;
 __global__ void __launch_bounds__(kThreads)
     embed_join_kernel(float* __restrict__ dw, long long ldw, EmbedWs ws, long long chunks, int slabs, int H, float scale,
                       int accumulate) {
-  constexpr int kJoinWarps = kThreads / 32, B = 4;  // pieces in flight
+  constexpr int B = 4;  // pieces in flight
   static_assert(kThreads == kSlab, "a thread per column");
   __shared__ float sum[kJoinWarps][kSlab];
+  __shared__ int s_pieces[kJoinWarps], s_id[kJoinWarps];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunk = static_cast<int>(blockIdx.x / slabs);
-  const int col0 = static_cast<int>(blockIdx.x - static_cast<long long>(chunk) * slabs) * kSlab;
-  const int valid = ws.start[ws.slots()];
-  const int next = (chunk + 1) * kChunk;
-  const int slot = ws.key[next];  // there is a chunk behind this one
-  if (next >= valid || ws.key[next - 1] != slot) return;
-  const int s = ws.start[slot], e = ws.start[slot + 1];
-  if (s < next - kChunk) return;  // it began earlier
-  const int m = (e - 1) / kChunk - chunk + 1;
+  const int chunk0 = static_cast<int>(blockIdx.x / slabs) * kJoinWarps;
+  const int col0 = static_cast<int>(blockIdx.x % slabs) * kSlab;
+  // acc = pieces first, first + step, ... of the m that begin in chunk c
   float acc[kLaneColumns];
+  auto add = [&](int c, int m, int first, int step) {
 #pragma unroll
-  for (int j = 0; j < kLaneColumns; ++j) acc[j] = 0.f;
-  for (int i0 = warp; i0 < m; i0 += B * kJoinWarps) {
-    float x[B][kLaneColumns];
+    for (int j = 0; j < kLaneColumns; ++j) acc[j] = 0.f;
+    for (int i0 = first; i0 < m; i0 += B * step) {
+      float x[B][kLaneColumns];
 #pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const int i = i0 + u * kJoinWarps;
-      const float* p = ws.part + ((i == 0 ? chunks : 0) + chunk + i) * H + col0 + lane;  // the first lies in slot 1
+      for (int u = 0; u < B; ++u) {
+        const int i = i0 + u * step;
+        const float* p = ws.part + ((i == 0 ? chunks : 0) + c + i) * H + col0 + lane;  // the first lies in slot 1
 #pragma unroll
-      for (int j = 0; j < kLaneColumns; ++j) x[u][j] = i < m && col0 + lane + 32 * j < H ? p[32 * j] : 0.f;
+        for (int j = 0; j < kLaneColumns; ++j) x[u][j] = i < m && col0 + lane + 32 * j < H ? p[32 * j] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+#pragma unroll
+        for (int j = 0; j < kLaneColumns; ++j) acc[j] += x[u][j];
     }
-#pragma unroll
-    for (int u = 0; u < B; ++u)
-#pragma unroll
-      for (int j = 0; j < kLaneColumns; ++j) acc[j] += x[u][j];
+  };
+  const int chunk = chunk0 + warp, next = (chunk + 1) * kChunk;
+  int pieces = 0, slot = 0;
+  if (chunk + 1 < chunks) {
+    const int valid = ws.start[ws.slots()], last = ws.key[next - 1];
+    slot = ws.key[next];
+    if (next < valid && last == slot && ws.start[slot] >= next - kChunk)
+      pieces = (ws.start[slot + 1] - 1) / kChunk - chunk + 1;
   }
+  const int id = pieces > 0 ? ws.id_of(slot) : 0;
+  if (pieces > 0 && pieces <= kOwnPieces) {
+    add(chunk, pieces, 0, 1);
 #pragma unroll
-  for (int j = 0; j < kLaneColumns; ++j) sum[warp][lane + 32 * j] = acc[j];
+    for (int j = 0; j < kLaneColumns; ++j) {
+      const int c = col0 + lane + 32 * j;
+      const float one[1] = {acc[j]};
+      if (c < H) emit_row<1>(dw + id * ldw + c, one, scale, accumulate);
+    }
+  }
+  if (lane == 0) {
+    s_pieces[warp] = pieces > kOwnPieces ? pieces : 0;
+    s_id[warp] = id;
+  }
   __syncthreads();
-  if (col0 + threadIdx.x >= H) return;
-  float v[1] = {0.f};
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const int m = s_pieces[w];
+    if (m == 0) continue;
+    add(chunk0 + w, m, warp, kJoinWarps);
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) v[0] += sum[w][threadIdx.x];
-  emit_row<1>(dw + ws.id_of(slot) * ldw + col0 + threadIdx.x, v, scale, accumulate);
+    for (int j = 0; j < kLaneColumns; ++j) sum[warp][lane + 32 * j] = acc[j];
+    __syncthreads();
+    const int c = col0 + threadIdx.x;
+    if (c < H) {
+      float one[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < kJoinWarps; ++i) one[0] += sum[i][threadIdx.x];
+      emit_row<1>(dw + s_id[w] * ldw + c, one, scale, accumulate);
+    }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -736,7 +766,8 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
   });
   REVPP_CHECK_LAUNCH();
   if (p.chunks < 2) return;  // no run crosses chunks
-  launch_pdl(embed_join_kernel, dim3(static_cast<unsigned>((p.chunks - 1) * p.slabs)), dim3(kThreads), 0, cur_stream(),
+  const long long joins = (p.chunks - 1 + kJoinWarps - 1) / kJoinWarps * p.slabs;
+  launch_pdl(embed_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(kThreads), 0, cur_stream(),
              dw.data_ptr<float>(), static_cast<long long>(dw.stride(0)), ws, p.chunks, p.slabs, H,
              static_cast<float>(scale), accumulate ? 1 : 0);
   REVPP_CHECK_LAUNCH();
