@@ -347,7 +347,8 @@ __device__ __forceinline__ void emit_row(float* __restrict__ dst, const float (&
     store_f32<V>(dst, o);
     return;
   }
-  // one addition per element and call: the order of the atomics does not matter
+  // One addition per element and call, so the order of the atomics does not matter; they need no
+  // read of dW here, and flush subnormal sums to zero.
   if constexpr (V % 4 == 0) {
 #pragma unroll
     for (int j = 0; j < V; j += 4)
@@ -610,6 +611,16 @@ void check_same_device(const torch::Tensor& a, const torch::Tensor& b, const cha
   REVPP_CHECK(a.device() == b.device(), names, " must be on the same device");
 }
 
+// A written tensor must lie apart from what is read.
+void check_apart(const torch::Tensor& written, const torch::Tensor& read, const char* names) {
+  auto end = [](const torch::Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size();
+  };
+  REVPP_CHECK(end(written) <= reinterpret_cast<uintptr_t>(read.data_ptr()) ||
+                  end(read) <= reinterpret_cast<uintptr_t>(written.data_ptr()),
+              names, " must not overlap");
+}
+
 template <typename F>
 void by_float(at::ScalarType t, F&& f) {
   if (t == at::kFloat)
@@ -655,6 +666,7 @@ void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tens
   REVPP_CHECK(w.size(1) <= (1 << 30), "rows too wide");
   if (n == 0 || w.size(1) == 0) return;
   REVPP_CHECK(vocab > 0, "the table is empty");
+  check_apart(out, w, "out and w");
   check_same_device(ids, w, "ids and w");
   check_same_device(w, out, "w and out");
   c10::cuda::CUDAGuard guard(w.device());
@@ -711,6 +723,7 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
               ", ", dy.size(1), "]");
   REVPP_CHECK(n < (1LL << 26) && vocab < (1LL << 30) && dw.size(1) < (1LL << 30), "too many tokens, rows or columns");
   if (vocab == 0 || dw.size(1) == 0 || (n == 0 && accumulate)) return;
+  if (n > 0) check_apart(dw, dy, "dw and dy");
   check_same_device(dy, dw, "dy and dw");
   check_same_device(ids, dw, "ids and dw");
   c10::cuda::CUDAGuard guard(dw.device());

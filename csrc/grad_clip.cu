@@ -322,28 +322,28 @@ torch::Tensor clip_grads(const py::list& grads, double max_norm, const c10::opti
     REVPP_CHECK(THPVariable_Check(o), name, " ", i, " is not a tensor");
     return THPVariable_Unpack(o);
   };
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    const torch::Tensor &g = tensor(grads.ptr(), i, "gradient"), &o = tensor(outs, i, "out");
-    REVPP_CHECK(type_of(g) >= 0 && type_of(o) >= 0, "tensor ", i, " must be float32, bfloat16 or float16");
-    REVPP_CHECK(g.layout() == at::kStrided && o.layout() == at::kStrided, "tensor ", i, " must be dense");
-    REVPP_CHECK(g.is_contiguous() || g.is_non_overlapping_and_dense(), "gradient ", i,
-                " has gaps or repeats in memory: make it contiguous");
-    REVPP_CHECK(same_layout(g, o), "out ", i, " must have its gradient's sizes and strides");
-  }
   std::vector<Entry> es;
   std::vector<int> indexes;
   es.reserve(n);
   indexes.reserve(n);
   const torch::Tensor& front = tensor(grads.ptr(), 0, "gradient");
+  const at::Device device = front.device();
   for (Py_ssize_t i = 0; i < n; ++i) {
     const torch::Tensor &g = tensor(grads.ptr(), i, "gradient"), &o = tensor(outs, i, "out");
+    const int gt = type_of(g), ot = type_of(o);
+    REVPP_CHECK(gt >= 0 && ot >= 0, "tensor ", i, " must be float32, bfloat16 or float16");
+    REVPP_CHECK(g.layout() == at::kStrided && o.layout() == at::kStrided, "tensor ", i, " must be dense");
+    REVPP_CHECK(g.is_contiguous() || g.is_non_overlapping_and_dense(), "gradient ", i,
+                " has gaps or repeats in memory: make it contiguous");
+    REVPP_CHECK(g.is_same(o) || same_layout(g, o), "out ", i, " must have its gradient's sizes and strides");
     REVPP_CHECK(g.is_cuda(), "gradient ", i, " must be a CUDA tensor");
-    REVPP_CHECK(g.device() == front.device() && o.device() == g.device(), "all tensors must be on one device");
-    if (g.numel() == 0) continue;
-    const void* src = g.data_ptr();
+    REVPP_CHECK(g.device() == device && o.device() == device, "all tensors must be on one device");
+    const int64_t count = g.numel();
+    if (count == 0) continue;
+    const void* src = g.const_data_ptr();
     void* dst = o.data_ptr();
     const bool wide = (reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) % 16 == 0;
-    es.push_back({src, dst, g.numel(), 0, static_cast<unsigned char>(type_of(g)), static_cast<unsigned char>(type_of(o)),
+    es.push_back({src, dst, count, 0, static_cast<unsigned char>(gt), static_cast<unsigned char>(ot),
                   static_cast<unsigned char>(wide), 0});
     indexes.push_back(static_cast<int>(i));
   }

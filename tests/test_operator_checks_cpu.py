@@ -14,6 +14,9 @@ def _ops():
     return ops
 
 
+SHARED = torch.zeros(8, 8)
+
+
 def _embed(**kw):
     a = dict(ids=torch.zeros(4, dtype=torch.long), w=torch.zeros(5, 8), out=torch.zeros(4, 8))
     a.update(kw)
@@ -25,7 +28,7 @@ def _embed(**kw):
     (dict(w=torch.zeros(5, 8, dtype=torch.float64)), "w must be"), (dict(w=torch.zeros(8)), "w must be 2-D"),
     (dict(w=torch.zeros(8, 5).t()), "contiguous along"), (dict(out=torch.zeros(3, 8)), "out must be"),
     (dict(out=torch.zeros(4, 9)), "out must be"), (dict(out=torch.zeros(1, 8).expand(4, 8)), "overlap"),
-    (dict(w=torch.zeros(0, 8)), "empty"), ({}, "CUDA")])
+    (dict(w=torch.zeros(0, 8)), "empty"), (dict(w=SHARED[:5], out=SHARED[4:8]), "must not overlap"), ({}, "CUDA")])
 def test_lookup_refuses(kw, message):
     with pytest.raises(RuntimeError, match=message):
         _ops().embedding_fwd(**_embed(**kw))
@@ -36,7 +39,7 @@ def test_lookup_refuses(kw, message):
     (dict(dy=torch.zeros(4, 8, dtype=torch.int32)), RuntimeError, "dy must be"),
     (dict(dy=torch.zeros(5, 8)), RuntimeError, "dy must be"), (dict(dw=torch.zeros(5, 9)), RuntimeError, "dy must be"),
     (dict(dw=torch.zeros(1, 8).expand(5, 8)), RuntimeError, "overlap"),
-    (dict(padding_idx=5), ValueError, "padding_idx"), (dict(padding_idx=-6), ValueError, "padding_idx"),
+    (dict(dy=SHARED[:4], dw=SHARED[3:8]), RuntimeError, "must not overlap"), (dict(padding_idx=5), ValueError, "padding_idx"), (dict(padding_idx=-6), ValueError, "padding_idx"),
     ({}, RuntimeError, "CUDA")])
 def test_gradient_refuses(kw, error, message):
     a = dict(dy=torch.zeros(4, 8), ids=torch.zeros(4, dtype=torch.int32), dw=torch.zeros(5, 8))
