@@ -83,7 +83,8 @@ def _tokens(kind, n, vocab, g):
     ("uniform", 1, 1, 1), ("uniform", 1, 3, 64), ("uniform", 31, 5, 40), ("uniform", 32, 2, 128), ("uniform", 33, 40, 13),
     ("skewed", 1000, 300, 128), ("skewed", 4097, 30522, 64), ("skewed", 9999, 257, 515), ("uniform", 700, 131072, 16),
     ("one", 33, 4, 32), ("one", 64, 1, 24), ("one", 1024, 3, 16), ("one", 1025, 3, 16), ("one", 9001, 200, 72),
-    ("skewed", 40000, 2, 256), ("uniform", 5000, 149, 1032), ("skewed", 300001, 500, 8), ("one", 140000, 9, 8)])
+    ("skewed", 40000, 2, 256), ("uniform", 5000, 149, 1032), ("skewed", 300001, 500, 8), ("one", 140000, 9, 8),
+    ("one", 256, 3, 130), ("skewed", 255, 40, 1024), ("skewed", 257, 40, 64), ("uniform", 200, 700, 67), ("skewed", 256, 90, 6)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_gradient(kind, n, vocab, width, dtype, accumulate):
