@@ -22,6 +22,13 @@
 //     piece per chunk in the workspace.  Without accumulation, further CTAs write zeros to the rows
 //     that no token names.
 //  3. embed_join_kernel: adds the pieces of each run that crosses chunks, in chunk order.
+//
+// What bounds them, and what they take at 32768 tokens x 1024 columns (B200, 30522 rows, a quarter of
+// the tokens padding): the lookup of fp32 rows into bf16 20 us, DRAM; the sort 10 us, latency (two
+// sweeps of dependent loads, shared-memory counters, a scan); the reduce 29 us when adding (137 MB,
+// 4.7 TB/s) and 41 us when writing every row, DRAM; the join 5.6 us, latency.  In the reduce all rows
+// of a warp (8 tokens x 1 KB) are loaded before the first is added: 20 warps per SM keep 160 KB in
+// flight; 16 tokens per warp left 12 warps and took 38 us, 8 of 32 tokens at a time 46 us.
 #include <algorithm>
 #include <atomic>
 
@@ -39,6 +46,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kFwdUnroll = 4;      // vectors per lane and row slab
+constexpr int kFwdBlocksPerSm = 4;
 constexpr int kSortWarps = 32;
 constexpr int kSortPer = 1024;     // tokens a warp lists at most before they are placed
 constexpr int kSortCluster = 4;    // CTAs that share a bin of ids, each with a part of the tokens
@@ -53,54 +61,61 @@ constexpr int kSlab = 32 * kLaneColumns;
 constexpr int kZeroRows = 8;       // dW rows per zero-writing warp
 
 // ------------------------------------------------------------------ forward
-// L lanes (a power of two) per (row, slab of L * V * kFwdUnroll columns).
+// L lanes (a power of two) per (row, slab of L * V * kFwdUnroll columns).  A group walks over its
+// pieces with the next one's id already on its way, so that a row costs one trip to memory, not two.
 template <typename TI, typename TW, typename TO, int V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kFwdBlocksPerSm)
     embed_fwd_kernel(const TI* __restrict__ ids, const TW* __restrict__ w, long long ldw, TO* __restrict__ out,
                      long long ldo, long long n, long long vocab, int H, int log_l, int slabs, float scale,
                      int* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
-  const long long group = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> log_l;
-  const int sub = threadIdx.x & ((1 << log_l) - 1);
-  const long long row = group / slabs;
-  if (row >= n) return;
-  const int slab = static_cast<int>(group - row * slabs);
-  const long long id = static_cast<long long>(ids[row]);
-  const bool ok = id >= 0 && id < vocab;
-  if (!ok && sub == 0 && slab == 0) atomicOr(status, kStatusBadShape);
-  const TW* src = w + (ok ? id : 0) * ldw;
-  TO* dst = out + row * ldo;
-  const int c0 = ((slab * kFwdUnroll << log_l) + sub) * V;
   constexpr int P = V * sizeof(TW) <= 16 ? V : 16 / sizeof(TW), Q = V * sizeof(TO) <= 16 ? V : 16 / sizeof(TO);
-  Pack<TW, P> x[kFwdUnroll][V / P];
+  const long long pieces = n * slabs, groups = (static_cast<long long>(gridDim.x) * kThreads) >> log_l;
+  long long piece = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> log_l;
+  const int sub = threadIdx.x & ((1 << log_l) - 1);
+  long long row = piece / slabs;
+  long long next_id = piece < pieces ? static_cast<long long>(ids[row]) : 0;
+  while (piece < pieces) {
+    const int slab = static_cast<int>(piece - row * slabs);
+    const long long id = next_id;
+    const bool ok = id >= 0 && id < vocab;
+    if (!ok && sub == 0 && slab == 0) atomicOr(status, kStatusBadShape);
+    const TW* src = w + (ok ? id : 0) * ldw;
+    TO* dst = out + row * ldo;
+    piece += groups;
+    row = piece / slabs;
+    if (piece < pieces) next_id = static_cast<long long>(ids[row]);
+    const int c0 = ((slab * kFwdUnroll << log_l) + sub) * V;
+    Pack<TW, P> x[kFwdUnroll][V / P];
 #pragma unroll
-  for (int u = 0; u < kFwdUnroll; ++u) {
-    const int c = c0 + ((u * V) << log_l);
+    for (int u = 0; u < kFwdUnroll; ++u) {
+      const int c = c0 + ((u * V) << log_l);
 #pragma unroll
-    for (int i = 0; i < V / P; ++i)
-      if (c < H && ok) x[u][i] = Pack<TW, P>::load_ro(src + c + i * P);
-  }
-#pragma unroll
-  for (int u = 0; u < kFwdUnroll; ++u) {
-    const int c = c0 + ((u * V) << log_l);
-    if (c >= H) continue;
-    float f[V];
-#pragma unroll
-    for (int i = 0; i < V / P; ++i) {
-      float g[P];
-      x[u][i].get(g);
-#pragma unroll
-      for (int j = 0; j < P; ++j) f[i * P + j] = ok ? g[j] * scale : 0.f;
+      for (int i = 0; i < V / P; ++i)
+        if (c < H && ok) x[u][i] = Pack<TW, P>::load_ro(src + c + i * P);
     }
 #pragma unroll
-    for (int i = 0; i < V / Q; ++i) {
-      float g[Q];
+    for (int u = 0; u < kFwdUnroll; ++u) {
+      const int c = c0 + ((u * V) << log_l);
+      if (c >= H) continue;
+      float f[V];
 #pragma unroll
-      for (int j = 0; j < Q; ++j) g[j] = f[i * Q + j];
-      Pack<TO, Q> y;
-      y.set(g);
-      y.store(dst + c + i * Q);
+      for (int i = 0; i < V / P; ++i) {
+        float g[P];
+        x[u][i].get(g);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[i * P + j] = ok ? g[j] * scale : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < V / Q; ++i) {
+        float g[Q];
+#pragma unroll
+        for (int j = 0; j < Q; ++j) g[j] = f[i * Q + j];
+        Pack<TO, Q> y;
+        y.set(g);
+        y.store(dst + c + i * Q);
+      }
     }
   }
 }
@@ -831,8 +846,7 @@ void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tens
   const int per_slab = (kFwdUnroll << log_l) * v;
   const int slabs = (H + per_slab - 1) / per_slab;
   const long long threads = (n * slabs) << log_l;
-  const long long blocks = (threads + kThreads - 1) / kThreads;
-  REVPP_CHECK(blocks < (1LL << 31), "too many tokens");
+  const long long blocks = std::min<long long>((threads + kThreads - 1) / kThreads, kFwdBlocksPerSm * num_sms());
   int* status = status_device_ptr();
   by_float(w.scalar_type(), [&](auto tw) {
     using TW = decltype(tw);

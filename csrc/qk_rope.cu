@@ -19,6 +19,11 @@
 //    with one set of angles;
 //  - bwd: one head, its vectors copied into shared memory two rows ahead (cp.async, every lane its
 //    own, so no barrier), since the registers are taken by weights and their gradients.
+// Value heads have no arithmetic; as lanes of their own they would be through early and leave warps
+// idle, so all lanes copy them at the end.  32768 rows of 16 heads x 64 bf16 (B200, out of place): fwd
+// 67 us, 403 MB at 0.91 of the copy rate (one head at a time with the next row prefetched 83 us); bwd
+// 103 us, 537 MB at 0.79 (two heads at once 128 us: registers for 12 warps per SM only; value heads as
+// lanes of their own 120 us).
 #include <algorithm>
 #include <atomic>
 
@@ -295,6 +300,11 @@ __device__ __forceinline__ long long checked(const QkArgs& a, long long pos) {
   return -1;
 }
 
+struct WeightGrads {
+  float *q, *k;
+  int accumulate;
+};
+
 template <typename T, int V, int U>
 struct Vectors {
   Pack<T, V> a[U], b[U];
@@ -447,10 +457,11 @@ struct Ring {
 };
 
 // part: [gridDim.x][2][dim] sums of dz x r over the block's query heads and key heads, added up
-// by qk_weight_grad_kernel in block order.
+// by qk_weight_grad_kernel in block order.  A single block writes dwq and dwk itself.
 template <typename T, int V, int U, bool NEIGHBOURS, bool FULL>
 __global__ void __launch_bounds__(kThreads, 2)
-    qk_norm_rope_bwd_kernel(const T* dy, const T* __restrict__ x, T* dx, QkArgs a, float* __restrict__ part) {
+    qk_norm_rope_bwd_kernel(const T* dy, const T* __restrict__ x, T* dx, QkArgs a, float* __restrict__ part,
+                            WeightGrads dw) {
   extern __shared__ __align__(16) char shared[];  // the rings, then [sets in the block][dim] sums
   pdl_wait();
   pdl_trigger();
@@ -543,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   copy_wait<0>();
   if (a.copies) copy_values<T, V>(dy, a.ldy, dx, a.lddx, a);
-  if (part == nullptr) return;
+  if (part == nullptr && dw.q == nullptr && dw.k == nullptr) return;
   __syncthreads();  // the rings give way to the sums
   float* sums = reinterpret_cast<float*>(shared);
   const int sets = a.groups * (kThreads / 32);  // of the block
@@ -569,14 +580,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       if ((set >= a.q_sets) == keys) v += sums[g * a.dim + column];
       if (++set == a.sets) set = 0;
     }
-    part[static_cast<long long>(blockIdx.x) * 2 * a.dim + c] = v;
+    if (part != nullptr) {
+      part[static_cast<long long>(blockIdx.x) * 2 * a.dim + c] = v;
+    } else if (float* d = keys ? dw.k : dw.q; d != nullptr) {
+      d[column] = dw.accumulate ? d[column] + v : v;
+    }
   }
 }
 
 // dw (+)= sums of part over the blocks, in a fixed order: 32 columns per block, 32 slices.
 __global__ void __launch_bounds__(1024)
-    qk_weight_grad_kernel(const float* __restrict__ part, int blocks, int dim, float* __restrict__ dwq,
-                          float* __restrict__ dwk, int accumulate) {
+    qk_weight_grad_kernel(const float* __restrict__ part, int blocks, int dim, WeightGrads dw) {
   __shared__ float s[32][33];
   pdl_wait();
   pdl_trigger();
@@ -591,10 +605,10 @@ __global__ void __launch_bounds__(1024)
   v = 0.f;
 #pragma unroll
   for (int i = 0; i < 32; ++i) v += s[i][lane];
-  float* d = c < dim ? dwq : dwk;
+  float* d = c < dim ? dw.q : dw.k;
   if (d == nullptr) return;
   const int col = c < dim ? c : c - dim;
-  d[col] = accumulate ? d[col] + v : v;
+  d[col] = dw.accumulate ? d[col] + v : v;
 }
 
 // ------------------------------------------------------------------ host
@@ -758,12 +772,13 @@ int resident(int device) {
   return n;
 }
 
-// Blocks for one resident wave, or fewer when the rows need fewer.
+// Blocks for one resident wave, or fewer when the rows need fewer; one where `single` would do.
 template <auto Kernel, int Smem>
-int blocks_for(const QkArgs& a, int device) {
+int blocks_for(const QkArgs& a, int device, int single) {
   const int per_block = a.groups * (kThreads / 32);
   const long long need = (static_cast<long long>(a.rows) * a.sets + per_block - 1) / per_block;
   const long long least = (a.sets + per_block - 1) / per_block;
+  if (least == 1 && need <= single) return 1;
   const long long wave = static_cast<long long>(resident<Kernel, Smem>(device)) * num_sms();
   return static_cast<int>(std::max(least, std::min(need, wave)));
 }
@@ -819,7 +834,7 @@ void qk_norm_rope_fwd(const torch::Tensor& qkv, torch::Tensor out, int64_t heads
     using T = decltype(e);
     constexpr auto kernel =
         &qk_norm_rope_fwd_kernel<T, decltype(v)::value, decltype(u)::value, kFwdHeads, decltype(nb)::value, decltype(full)::value>;
-    launch_pdl(kernel, dim3(blocks_for<kernel, 0>(a, qkv.get_device())), dim3(kThreads), 0, cur_stream(),
+    launch_pdl(kernel, dim3(blocks_for<kernel, 0>(a, qkv.get_device(), 1)), dim3(kThreads), 0, cur_stream(),
                static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(out.data_ptr()), a);
   });
   REVPP_CHECK_LAUNCH();
@@ -851,6 +866,8 @@ void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch
   check_devices(qkv, {&dout, &dqkv, ptr_of(wq), ptr_of(wk), ptr_of(dwq), ptr_of(dwk), ptr_of(cos), ptr_of(sin),
                       ptr_of(positions)});
   c10::cuda::CUDAGuard guard(qkv.device());
+  const WeightGrads dw{given(dwq) ? dwq->data_ptr<float>() : nullptr, given(dwk) ? dwk->data_ptr<float>() : nullptr,
+                       accumulate ? 1 : 0};
   int blocks = 0;
   torch::Tensor part;
   if (a.rows > 0) {
@@ -864,19 +881,19 @@ void qk_norm_rope_bwd(const torch::Tensor& dout, const torch::Tensor& qkv, torch
       constexpr auto kernel =
           &qk_norm_rope_bwd_kernel<T, decltype(v)::value, decltype(u)::value, decltype(nb)::value, decltype(full)::value>;
       constexpr int smem = kBwdSmem<T, decltype(v)::value, decltype(u)::value>;
-      blocks = blocks_for<kernel, smem>(a, qkv.get_device());
-      if (weights) part = torch::empty({static_cast<int64_t>(blocks) * 2 * a.dim}, qkv.options().dtype(at::kFloat));
+      // work for two blocks goes to one that needs no second launch for the weight gradients
+      blocks = blocks_for<kernel, smem>(a, qkv.get_device(), weights ? 2 : 1);
+      if (weights && blocks > 1) part = torch::empty({static_cast<int64_t>(blocks) * 2 * a.dim}, qkv.options().dtype(at::kFloat));
       launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, cur_stream(), static_cast<const T*>(dout.data_ptr()),
                  static_cast<const T*>(qkv.data_ptr()), static_cast<T*>(dqkv.data_ptr()), a,
-                 weights ? part.data_ptr<float>() : static_cast<float*>(nullptr));
+                 weights && blocks > 1 ? part.data_ptr<float>() : static_cast<float*>(nullptr), dw);
     });
     REVPP_CHECK_LAUNCH();
   }
-  if (!weights) return;
+  if (!weights || blocks == 1) return;
   launch_pdl(qk_weight_grad_kernel, dim3((2 * a.dim + 31) / 32), dim3(1024), 0, cur_stream(),
              blocks > 0 ? const_cast<const float*>(part.data_ptr<float>()) : static_cast<const float*>(nullptr), blocks, a.dim,
-             given(dwq) ? dwq->data_ptr<float>() : static_cast<float*>(nullptr),
-             given(dwk) ? dwk->data_ptr<float>() : static_cast<float*>(nullptr), accumulate ? 1 : 0);
+             dw);
   REVPP_CHECK_LAUNCH();
 }
 
