@@ -730,6 +730,8 @@ void finish(Problem& p, std::initializer_list<const torch::Tensor*> packed, cons
   else
     a.units = half / v + ((a.dim - a.rot) / v + 1) / 2;
   // One unit per lane, or (narrow vectors) as many as leave fewer lanes idle; heads do not cross warps.
+  // 12 + 6 heads of 72 columns, 36 of them rotated, fp32, backward: 18 units on 18 lanes of a warp take
+  // 61 us, two units each on 9 lanes, three heads to a warp, 32 us.
   auto lanes = [&](int u) { return (a.units + u - 1) / u; };
   p.u = v == 2 ? 2 : v == 1 ? 4 : 1;
   if (lanes(1) <= 32 && (p.u == 1 || (32 / lanes(1)) * p.u >= 32 / lanes(p.u))) p.u = 1;
