@@ -11,8 +11,8 @@
 // and every dW row is written once, so equal inputs give equal bits.
 //
 //  1. embed_sort_kernel: 2^c bins, each of the ids with the same low c bits (frequent tokens, which
-//     vocabularies number low, spread over the bins).  A cluster of four CTAs per bin reads all n ids,
-//     a quarter each, counts those of earlier bins (the bin's offset in the sorted order, with no
+//     vocabularies number low, spread over the bins).  A cluster of four CTAs per bin (two or one where
+//     the table has more than 32768 or 65536 rows) reads all n ids, a part each, counts those of earlier bins (the bin's offset in the sorted order, with no
 //     exchange between clusters) and places its own by a counting sort: the CTAs' counts meet over
 //     distributed shared memory, and within a CTA up to 16 warps take consecutive parts of its tokens,
 //     so that the order within an id is the token order.
@@ -49,8 +49,8 @@ constexpr int kFwdUnroll = 4;      // vectors per lane and row slab
 constexpr int kFwdBlocksPerSm = 4;
 constexpr int kSortWarps = 32;
 constexpr int kSortPer = 1024;     // tokens a warp lists at most before they are placed
-constexpr int kSortCluster = 4;    // CTAs that share a bin of ids, each with a part of the tokens
-constexpr int kSortLogBins = 5;    // at most one CTA per SM, unless the table is very long
+constexpr int kSortCtas = 128;     // at most one CTA per SM, unless the table is very long
+constexpr int kSortCluster = 4;    // CTAs that share a bin of ids, each with a part of the tokens; fewer for long tables
 constexpr int kSortLogRange = 10;  // ids per bin: 1024 at most, one per thread
 constexpr int kRankers = 16;       // warps that place tokens
 constexpr int kWarps = 4;          // of a reduce CTA
@@ -212,8 +212,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
   return v;
 }
 
-template <typename TI>
-__global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarps * 32, 1)
+template <typename TI, int C>
+__global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(kSortWarps * 32, 1)
     embed_sort_kernel(const TI* __restrict__ ids, int n, int per, unsigned vocab, unsigned padding, EmbedWs ws,
                       int* __restrict__ status) {
   // [kSortWarps][per] tokens of each warp, [kRankers][range] next positions of each ranking warp
@@ -225,9 +225,9 @@ __global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarp
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int range = 1 << ws.log_r;
   const int rank = static_cast<int>(cluster.block_rank());
-  const int bin = blockIdx.x / kSortCluster;
+  const int bin = blockIdx.x / C;
   const int share = kSortWarps * per;           // tokens of a CTA whose lists fit into shared memory
-  const int segment = kSortCluster * share;
+  const int segment = C * share;
   const int slot = threadIdx.x;                 // the thread's local id, where slot < range
   int* list = sm + warp * per;
   int* hist = sm + kSortWarps * per;
@@ -249,7 +249,7 @@ __global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarp
     int total = 0;
     earlier = 0;
 #pragma unroll
-    for (int r = 0; r < kSortCluster; ++r) {
+    for (int r = 0; r < C; ++r) {
       const int c = cluster.map_shared_rank(s_count, r)[slot];
       total += c;
       earlier += r < rank ? c : 0;
@@ -266,7 +266,7 @@ __global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarp
   const int total = gather(earlier);
   int base = 0;
 #pragma unroll
-  for (int r = 0; r < kSortCluster; ++r) base += cluster.map_shared_rank(s_less, r)[lane];
+  for (int r = 0; r < C; ++r) base += cluster.map_shared_rank(s_less, r)[lane];
   base = warp_sum(base);
   const int incl = warp_scan(total, lane);
   if (lane == 31) s_sum[warp] = incl;
@@ -276,7 +276,7 @@ __global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortWarp
   s_next[slot] = first + (many ? 0 : earlier);
   if (rank == 0 && slot < range) {
     ws.start[bin * range + slot] = first;
-    if (blockIdx.x + kSortCluster >= gridDim.x && slot == range - 1) ws.start[ws.slots()] = first + total;
+    if (blockIdx.x + C >= gridDim.x && slot == range - 1) ws.start[ws.slots()] = first + total;
   }
   for (long long seg = 0; seg < n; seg += segment) {
     int of_segment = 0;
@@ -798,17 +798,18 @@ void by_float(at::ScalarType t, F&& f) {
 long long align256(long long b) { return (b + 255) / 256 * 256; }
 
 struct Plan {
-  int v, slabs, log_c, log_r;
+  int v, slabs, log_c, log_r, cluster;
   long long chunks, off_order, off_key, off_part, bytes;
 };
 Plan plan_bwd(long long n, long long vocab, int H, int v) {
   Plan p;
   p.v = v;
   p.slabs = (H + kSlab - 1) / kSlab;
-  p.log_c = 0;
-  while (p.log_c < kSortLogBins && (1LL << p.log_c) < vocab) ++p.log_c;
-  p.log_r = 0;
+  p.log_c = p.log_r = 0;
+  while ((kSortCluster << p.log_c) < kSortCtas && (1LL << p.log_c) < vocab) ++p.log_c;
   while ((1LL << (p.log_c + p.log_r)) < vocab) ++(p.log_r < kSortLogRange ? p.log_r : p.log_c);
+  p.cluster = kSortCluster;
+  while (p.cluster > 1 && (static_cast<long long>(p.cluster) << p.log_c) > kSortCtas) p.cluster /= 2;
   p.chunks = (n + kChunk - 1) / kChunk;
   p.off_order = align256(((1LL << (p.log_c + p.log_r)) + 1) * 4);
   p.off_key = p.off_order + align256(n * 4);
@@ -842,7 +843,7 @@ void embedding_fwd(const torch::Tensor& ids, const torch::Tensor& w, torch::Tens
                     rows_allow(out, out.stride(0), n, std::min(v, out_most))))
     v /= 2;
   int log_l = 0;
-  while (log_l < 5 && (1 << log_l) * v < H) ++log_l;
+  while (log_l < 5 && (kFwdUnroll << log_l) * v < H) ++log_l;  // narrow rows: several per warp, all lanes loading
   const int per_slab = (kFwdUnroll << log_l) * v;
   const int slabs = (H + per_slab - 1) / per_slab;
   const long long threads = (n * slabs) << log_l;
@@ -934,24 +935,30 @@ void embedding_bwd(const torch::Tensor& dy, const torch::Tensor& ids, torch::Ten
              reinterpret_cast<int*>(base + p.off_key), reinterpret_cast<float*>(base + p.off_part), p.log_c, p.log_r};
   int* status = status_device_ptr();
   // the cluster's warps list all tokens, in segments where there are more than kSortPer for each
-  constexpr int kLists = kSortCluster * kSortWarps;
-  const int per = static_cast<int>(std::min<long long>(kSortPer, (n + kLists * 64 - 1) / (kLists * 64) * 64));
+  const int lists = p.cluster * kSortWarps * 64;
+  const int per = static_cast<int>(std::min<long long>(kSortPer, (n + lists - 1) / lists * 64));
   const size_t smem = (static_cast<size_t>(kRankers << p.log_r) + kSortWarps * per) * 4;
   const unsigned padding = padding_idx >= 0 && padding_idx < vocab ? static_cast<unsigned>(padding_idx) : 0xffffffffu;
-  auto sort = [&](auto ti) {
+  auto sort = [&](auto ti, auto cluster) {
     using TI = decltype(ti);
+    constexpr auto kernel = &embed_sort_kernel<TI, decltype(cluster)::value>;
     static std::atomic<uint64_t> ready{0};  // devices that know the kernel's shared memory
     const uint64_t bit = 1ull << (dw.get_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
-      REVPP_CUDA_CHECK(cudaFuncSetAttribute(embed_sort_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      REVPP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             ((kRankers << kSortLogRange) + kSortWarps * kSortPer) * 4));
       ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    launch_pdl(embed_sort_kernel<TI>, dim3(kSortCluster << p.log_c), dim3(kSortWarps * 32), smem, cur_stream(),
+    launch_pdl(kernel, dim3(static_cast<unsigned>(p.cluster) << p.log_c), dim3(kSortWarps * 32), smem, cur_stream(),
                static_cast<const TI*>(ids.data_ptr()), static_cast<int>(n), per, static_cast<unsigned>(vocab), padding, ws, status);
   };
-  if (ids.scalar_type() == at::kLong) sort(int64_t{});
-  else sort(int32_t{});
+  auto by_cluster = [&](auto ti) {
+    if (p.cluster == 4) sort(ti, std::integral_constant<int, 4>{});
+    else if (p.cluster == 2) sort(ti, std::integral_constant<int, 2>{});
+    else sort(ti, std::integral_constant<int, 1>{});
+  };
+  if (ids.scalar_type() == at::kLong) by_cluster(int64_t{});
+  else by_cluster(int32_t{});
   REVPP_CHECK_LAUNCH();
   const long long zero_rows = kWarps * kZeroRows;
   const long long blocks = p.chunks * p.slabs + (accumulate ? 0 : (vocab + zero_rows - 1) / zero_rows);

@@ -84,6 +84,7 @@ def _tokens(kind, n, vocab, g):
     ("skewed", 1000, 300, 128), ("skewed", 4097, 30522, 64), ("skewed", 9999, 257, 515), ("uniform", 700, 131072, 16),
     ("one", 33, 4, 32), ("one", 64, 1, 24), ("one", 1024, 3, 16), ("one", 1025, 3, 16), ("one", 9001, 200, 72),
     ("skewed", 40000, 2, 256), ("uniform", 5000, 149, 1032), ("skewed", 300001, 500, 8), ("one", 140000, 9, 8),
+    ("skewed", 3000, 40000, 24), ("skewed", 140001, 40000, 8), ("uniform", 3000, 131072, 8), ("skewed", 70000, 70000, 8), ("uniform", 900, 140000, 8),
     ("one", 256, 3, 130), ("skewed", 255, 40, 1024), ("skewed", 257, 40, 64), ("uniform", 200, 700, 67), ("skewed", 256, 90, 6)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("accumulate", [False, True])
