@@ -96,13 +96,70 @@ class StepLR:
             self.opt.lr *= self.gamma
 
 
+def _values(t: torch.Tensor) -> torch.Tensor:
+    """The strided tensor that holds the numbers of ``t``."""
+    if t.layout == torch.strided:
+        return t
+    return t._values() if t.layout == torch.sparse_coo else t.values()
+
+
+def _layout(t: torch.Tensor):
+    """Strides and sizes that count, the shortest stride first."""
+    return sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1)
+
+
+def _pieces(t: torch.Tensor):
+    """Where the contiguous pieces of ``t`` start (bytes, ascending), and how many bytes each has."""
+    dims, length, starts = _layout(t), 1, torch.zeros(1, dtype=torch.int64, device="cpu")
+    while dims and dims[0][0] == length:
+        length *= dims.pop(0)[1]
+    for st, n in dims:
+        starts = (starts[:, None] + st * torch.arange(n, device="cpu")).flatten()
+    return t.data_ptr() + t.element_size() * starts.sort().values, t.element_size() * length
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors whose spans overlap have a byte in common."""
+    if a.is_contiguous() and b.is_contiguous():
+        return True
+    (x, m), (y, n) = _pieces(a), _pieces(b)
+    at = torch.searchsorted(y, x + m)  # pieces of b that start before each piece of a ends
+    return bool(((at > 0) & (y[(at - 1).clamp_(min=0)] + n > x)).any())
+
+
+def _check_apart(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor]) -> None:
+    """Refuses outputs that share memory with another output, themselves or a gradient that is not their own."""
+    spans = []  # first byte, end, what it is, the tensor
+    for i, (g, o) in enumerate(zip(map(_values, grads), map(_values, outs))):
+        own = g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.shape == o.shape and all(
+            a == b for a, b, n in zip(g.stride(), o.stride(), g.shape) if n > 1)
+        for name, t in (("out", o),) if own else (("out", o), ("gradient", g)):
+            if t.numel():
+                last = sum(st * (n - 1) for n, st in zip(t.shape, t.stride()))
+                spans.append((t.data_ptr(), t.data_ptr() + t.element_size() * (last + 1), (name, i), t))
+        if not o.is_contiguous():
+            starts, length = _pieces(o)
+            if (starts.diff() < length).any():
+                raise ValueError(f"out {i} shares memory with itself: make it contiguous")
+    spans.sort(key=lambda s: s[:3])
+    reach = []  # earlier ones that end behind the present start
+    for s in spans:
+        reach = [a for a in reach if a[1] > s[0]]
+        for a in reach:
+            if "out" in (a[2][0], s[2][0]) and _share(a[3], s[3]):
+                raise ValueError("{} {} shares memory with {} {}: an output must be its own gradient, or lie apart from "
+                                 "all other tensors".format(*a[2], *s[2]))
+        reach.append(s)
+
+
 def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
                norm_type: float = 2.0) -> torch.Tensor:
     """Clip separate gradient tensors by their global norm, as ``FlatAdamW`` does for a flat buffer.
 
     For parameters that live outside ``FlatParams`` (modules split by ``parallel.tracer``): scales every
     gradient by min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (for instance the
-    ``FlatParams.grad_of`` views), and returns the norm (fp32 scalar).  CUDA tensors go through the
+    ``FlatParams.grad_of`` views), and returns the norm (fp32 scalar).  An output that shares memory with
+    another one, or with a gradient that is not its own, is refused.  CUDA tensors go through the
     kernels (``ops.clip_grads``), CPU tensors through PyTorch."""
     grads = list(grads)
     if not grads:
@@ -120,6 +177,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
         raise ValueError(f"out must have one tensor per gradient: {len(outs)} for {len(grads)}")
     if any(o.shape != g.shape for o, g in zip(outs, grads)):
         raise ValueError("out must have its gradients' sizes")
+    _check_apart(grads, outs)
     with torch.no_grad():
         full = [g.double() for g in grads if g.numel()]
         if norm_type == 2.0:

@@ -1,0 +1,61 @@
+"""Clipping of separate gradient tensors on the CPU against the definition in 64 bits."""
+import pytest
+import torch
+
+import operator_oracles as oracle
+from revpp import optim
+
+
+def _coef(grads, max_norm):
+    return min(1.0, max_norm / (torch.cat([g.double().reshape(-1) for g in grads]).norm().item() + 1e-6))
+
+
+def _refused(grads, out=None):
+    """Raises, and leaves everything as it was."""
+    tensors = list(grads) + list(out or [])
+    kept = [t.clone() for t in tensors]
+    with pytest.raises(ValueError, match="shares memory"):
+        optim.clip_grads(grads, 0.1, out=out)
+    assert all(torch.equal(t, k) for t, k in zip(tensors, kept))
+
+
+def test_outputs_that_share_memory_are_refused():
+    g, base = torch.ones(4), torch.arange(1.0, 41.0)
+    _refused([g, g])                                        # would be scaled twice
+    _refused([g, g.view(2, 2)])
+    _refused([base[:2], base[2:4]], out=[base[2:4], base[:2]])  # the second would be read after it was written
+    _refused([base[:10], base[5:20]])
+    _refused([base[:10]], out=[base[1:11]])
+    _refused([base[:10]], out=[base.view(torch.bfloat16)[:10]])
+    _refused([g, torch.zeros(4)], out=[base[:4], base[3:7]])
+    _refused([base.view(4, 10)[:, :5], base.view(4, 10)[:, 4:6]])
+    _refused([base.view(4, 10).t()], out=[base.view(10, 4)])
+    _refused([torch.ones(3, 4)], out=[base[:4].expand(3, 4)])
+    _refused([base[::2], base[::3]])
+
+
+def test_tensors_of_one_buffer_that_lie_apart():
+    base = torch.randn(24, 10)
+    pieces = [base[:, :5], base[:, 5:9], base[::2, 9], base[1::2, 9]]
+    kept, before = [p.clone() for p in pieces], base.clone()
+    optim.clip_grads(pieces, 0.5)
+    oracle.within(base, before.double() * _coef(kept, 0.5), before.double().abs() * 2 * oracle.U)
+    # sizes of one leave their strides open
+    row = base[:1]
+    optim.clip_grads([row], 1e6, out=[row.as_strided((1, 10), (3, 1))])
+    # one gradient twice counts twice, into two outputs of one buffer; empty tensors lie nowhere
+    g, buf = torch.randn(6), torch.zeros(12)
+    optim.clip_grads([g, g, torch.zeros(0)], 0.5, out=[buf[:6], buf[6:], buf[3:3]])
+    assert torch.equal(buf[:6], buf[6:])
+    oracle.within(buf[:6], g.double() * _coef([g, g], 0.5), g.double().abs() * 2 * oracle.U)
+
+
+def test_sparse_gradients():
+    net = torch.nn.Embedding(6, 3, sparse=True)
+    net(torch.tensor([1, 1, 2])).sum().backward()
+    dense = net.weight.grad.to_dense()
+    norm = optim.clip_grads([net.weight.grad, torch.ones(2)], 0.5)
+    assert abs(norm.item() - 17 ** 0.5) <= 2 * oracle.U * 17 ** 0.5  # rows of 2, 2, 2 and 1, 1, 1, and the ones
+    oracle.within(net.weight.grad.to_dense(), dense.double() * _coef([dense, torch.ones(2)], 0.5), dense.double() * 4 * oracle.U)
+    with pytest.raises(ValueError, match="shares memory"):
+        optim.clip_grads([net.weight.grad, net.weight.grad], 0.5)
