@@ -160,7 +160,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
     gradient by min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (for instance the
     ``FlatParams.grad_of`` views), and returns the norm (fp32 scalar).  An output that shares memory with
     another one, or with a gradient that is not its own, is refused.  CUDA tensors go through the
-    kernels (``ops.clip_grads``), CPU tensors through PyTorch."""
+    kernels (``ops.clip_grads``: fp32, bf16 and fp16), CPU tensors through PyTorch (float64 too)."""
     grads = list(grads)
     if not grads:
         return torch.zeros(())
@@ -184,9 +184,9 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
             norm = sum((g.square().sum() for g in full), torch.zeros((), dtype=torch.float64)).sqrt()
         else:
             norm = torch.stack([g.abs().max() for g in full]).max() if full else torch.zeros((), dtype=torch.float64)
-        coef = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
-        for g, o in zip(grads, outs):
-            o.copy_(g.float() * coef)
+        coef = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+        for g, o in zip(grads, outs):  # float64 gradients are scaled in 64 bits, the others in 32
+            o.copy_(g * coef if g.dtype == torch.float64 else g.float() * coef.float())
     return norm.float()
 
 

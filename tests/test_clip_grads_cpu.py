@@ -59,3 +59,28 @@ def test_sparse_gradients():
     oracle.within(net.weight.grad.to_dense(), dense.double() * _coef([dense, torch.ones(2)], 0.5), dense.double() * 4 * oracle.U)
     with pytest.raises(ValueError, match="shares memory"):
         optim.clip_grads([net.weight.grad, net.weight.grad], 0.5)
+
+
+@pytest.mark.parametrize("max_norm", [0.3, 1e6])
+def test_float64_gradients_keep_their_bits(max_norm):
+    torch.manual_seed(1)
+    grads = [torch.randn(50, dtype=torch.float64), torch.randn(9), torch.randn(7, dtype=torch.float64).to(torch.bfloat16)]
+    kept = [g.clone() for g in grads]
+    norm = optim.clip_grads(grads, max_norm)
+    coef = _coef(kept, max_norm)
+    assert norm.dtype == torch.float32
+    # norm and factor are computed in 64 bits: about 70 roundings of 2^-53, and the product's
+    oracle.within(grads[0], kept[0] * coef, (kept[0] * coef).abs() * 80 * 2.0 ** -53)
+    for g, k in zip(grads[1:], kept[1:]):
+        y = k.double() * coef
+        oracle.within(g, y, y.abs() * (2 * oracle.U + oracle.half_step(g.dtype)))
+    if max_norm == 1e6:
+        assert all(torch.equal(g, k) for g, k in zip(grads, kept))
+
+
+def test_float64_gradients_beyond_the_range_of_32_bits():
+    for big in (1e60, 1e-60):
+        grads = [torch.tensor([3.0, -4.0], dtype=torch.float64) * big, torch.zeros(2)]
+        optim.clip_grads(grads, big)
+        assert torch.allclose(grads[0], torch.tensor([3.0, -4.0], dtype=torch.float64) * big * (big / (5 * big + 1e-6)), rtol=1e-14, atol=0)
+        assert not grads[1].any()
