@@ -175,6 +175,10 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"out must have one tensor per gradient: {len(outs)} for {len(grads)}")
+    for name, tensors in (("gradient", grads), ("out", outs)):
+        for i, t in enumerate(tensors):
+            if not t.is_floating_point():
+                raise ValueError(f"{name} {i} must be a floating-point tensor, got {t.dtype}")
     if any(o.shape != g.shape for o, g in zip(outs, grads)):
         raise ValueError("out must have its gradients' sizes")
     _check_apart(grads, outs)

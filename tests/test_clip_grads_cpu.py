@@ -84,3 +84,13 @@ def test_float64_gradients_beyond_the_range_of_32_bits():
         optim.clip_grads(grads, big)
         assert torch.allclose(grads[0], torch.tensor([3.0, -4.0], dtype=torch.float64) * big * (big / (5 * big + 1e-6)), rtol=1e-14, atol=0)
         assert not grads[1].any()
+
+
+def test_types_without_a_fraction_or_with_an_imaginary_part_are_refused():
+    for bad in (torch.tensor([3, 4]), torch.tensor([3 + 4j]), torch.tensor([True])):
+        kept = bad.clone()
+        with pytest.raises(ValueError, match="gradient 1 must be a floating-point tensor"):
+            optim.clip_grads([torch.ones(2), bad], 1.0)
+        with pytest.raises(ValueError, match="out 0 must be a floating-point tensor"):
+            optim.clip_grads([torch.ones(bad.shape)], 1.0, out=[bad])
+        assert torch.equal(bad, kept)
