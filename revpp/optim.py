@@ -159,12 +159,13 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
     For parameters that live outside ``FlatParams`` (modules split by ``parallel.tracer``): scales every
     gradient by min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (for instance the
     ``FlatParams.grad_of`` views), and returns the norm (fp32 scalar).  An output that shares memory with
-    another one, or with a gradient that is not its own, is refused.  CUDA tensors go through the
+    another one, or with a gradient that is not its own, is refused, and so is a None in the lists
+    (parameters without a gradient have to be left out).  CUDA tensors go through the
     kernels (``ops.clip_grads``: fp32, bf16 and fp16), CPU tensors through PyTorch (float64 too)."""
     grads = list(grads)
     if not grads:
         return torch.zeros(())
-    if grads[0].is_cuda:
+    if isinstance(grads[0], torch.Tensor) and grads[0].is_cuda:
         from revpp import ops
 
         return ops.clip_grads(grads, max_norm, out, norm_type)
@@ -177,6 +178,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
         raise ValueError(f"out must have one tensor per gradient: {len(outs)} for {len(grads)}")
     for name, tensors in (("gradient", grads), ("out", outs)):
         for i, t in enumerate(tensors):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} {i} is not a tensor: {type(t).__name__}")
             if not t.is_floating_point():
                 raise ValueError(f"{name} {i} must be a floating-point tensor, got {t.dtype}")
     if any(o.shape != g.shape for o, g in zip(outs, grads)):

@@ -94,3 +94,18 @@ def test_types_without_a_fraction_or_with_an_imaginary_part_are_refused():
         with pytest.raises(ValueError, match="out 0 must be a floating-point tensor"):
             optim.clip_grads([torch.ones(bad.shape)], 1.0, out=[bad])
         assert torch.equal(bad, kept)
+
+
+def test_a_missing_gradient_is_named():
+    net = torch.nn.Linear(3, 2)
+    net.bias.requires_grad_(False)
+    net(torch.ones(1, 3)).sum().backward()
+    for grads in ([p.grad for p in net.parameters()], [None, torch.ones(2)]):
+        at = 1 if grads[0] is not None else 0
+        with pytest.raises(TypeError, match=f"gradient {at} is not a tensor: NoneType"):
+            optim.clip_grads(grads, 1.0)
+    with pytest.raises(TypeError, match="out 0 is not a tensor"):
+        optim.clip_grads([torch.ones(2)], 1.0, out=[None])
+    # the call for modules with frozen or unused parameters
+    norm = optim.clip_grads([p.grad for p in net.parameters() if p.grad is not None], 1.0)
+    assert abs(norm.item() - 6 ** 0.5) <= 2 * oracle.U * 6 ** 0.5
