@@ -182,6 +182,9 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
                 raise TypeError(f"{name} {i} is not a tensor: {type(t).__name__}")
             if not t.is_floating_point():
                 raise ValueError(f"{name} {i} must be a floating-point tensor, got {t.dtype}")
+            if t.device != grads[0].device:
+                raise ValueError(f"all tensors must be on one device: {name} {i} is on {t.device}, gradient 0 on "
+                                 f"{grads[0].device}")
     if any(o.shape != g.shape for o, g in zip(outs, grads)):
         raise ValueError("out must have its gradients' sizes")
     _check_apart(grads, outs)

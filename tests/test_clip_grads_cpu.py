@@ -109,3 +109,23 @@ def test_a_missing_gradient_is_named():
     # the call for modules with frozen or unused parameters
     norm = optim.clip_grads([p.grad for p in net.parameters() if p.grad is not None], 1.0)
     assert abs(norm.item() - 6 ** 0.5) <= 2 * oracle.U * 6 ** 0.5
+
+
+def test_tensors_of_several_devices_are_refused():
+    a, b = torch.ones(3), torch.ones(3, device="meta")
+    for grads, out in (([a, b], None), ([a, a.clone()], [torch.zeros(3), b]), ([a], [b])):
+        with pytest.raises(ValueError, match="on one device"):
+            optim.clip_grads(grads, 0.1, out=out)
+    assert (a == 1).all()
+
+
+@pytest.mark.gpu
+def test_cpu_and_cuda_tensors_in_one_list_are_refused():
+    a, b = torch.ones(3), torch.ones(3, device="cuda")
+    for grads, out in (([a, b], None), ([a], [b])):
+        with pytest.raises(ValueError, match="on one device"):
+            optim.clip_grads(grads, 0.1, out=out)
+    for grads, out in (([b, a], None), ([b], [a])):
+        with pytest.raises(RuntimeError, match="device|CUDA"):
+            optim.clip_grads(grads, 0.1, out=out)
+    assert (a == 1).all() and (b == 1).all()
