@@ -187,7 +187,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Seq
                                  f"{grads[0].device}")
     if any(o.shape != g.shape for o, g in zip(outs, grads)):
         raise ValueError("out must have its gradients' sizes")
-    _check_apart(grads, outs)
+    if not grads[0].is_meta:
+        _check_apart(grads, outs)
     with torch.no_grad():
         full = [g.double() for g in grads if g.numel()]
         if norm_type == 2.0:

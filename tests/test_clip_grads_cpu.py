@@ -129,3 +129,8 @@ def test_cpu_and_cuda_tensors_in_one_list_are_refused():
         with pytest.raises(RuntimeError, match="device|CUDA"):
             optim.clip_grads(grads, 0.1, out=out)
     assert (a == 1).all() and (b == 1).all()
+
+
+def test_tensors_without_memory_pass():
+    grads = [torch.ones(3, device="meta"), torch.ones(2, 2, device="meta")]
+    assert optim.clip_grads(grads, 1.0).shape == ()
