@@ -201,7 +201,9 @@ __device__ __forceinline__ void rotate(float (&xa)[V], float (&xb)[V], const flo
   }
 }
 
-// The lane's place: its heads, first row and row stride (rows advance by whole sets of heads).
+// The lane's place: its heads, first row and row stride (rows advance by whole sets of heads).  Row
+// counters are unsigned: those of a lane with nothing to do start at `rows` (below 2^30) and advance with
+// the others, two strides ahead of the last trip, which passes 2^31.
 struct Place {
   bool keys;
   int head, count;        // the first of `count` heads, among all of the row
@@ -283,7 +285,7 @@ struct Positions {
     }
   }
   // of `row`; rows come in order
-  __device__ __forceinline__ long long next(const QkArgs& a, int row) {
+  __device__ __forceinline__ long long next(const QkArgs& a, unsigned row) {
     if (a.pos != nullptr)
       return a.pos64 ? static_cast<const int64_t*>(a.pos)[row] : static_cast<const int32_t*>(a.pos)[row];
     const int now = at;
@@ -369,10 +371,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const T* xr = x + static_cast<long long>(p.row) * a.ldx + p.head * a.dim;
   T* yr = y + static_cast<long long>(p.row) * a.ldy + p.head * a.dim;
   const long long step_x = static_cast<long long>(p.stride) * a.ldx, step_y = static_cast<long long>(p.stride) * a.ldy;
-  const int trips = (a.rows + p.stride - 1) / p.stride;
-  int row = p.row;
-  for (int t = 0; t < trips; ++t, row += p.stride, xr += step_x, yr += step_y) {
-    const bool on = row < a.rows;
+  const unsigned rows = a.rows, trips = (rows + p.stride - 1) / p.stride;
+  unsigned row = p.row;
+  for (unsigned t = 0; t < trips; ++t, row += p.stride, xr += step_x, yr += step_y) {
+    const bool on = row < rows;
     Vectors<T, V, U> v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h)
@@ -482,9 +484,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   {
     const Ring<T, V, U> ring{shared};
-    int row = p.row, ahead = row;  // the row that is fetched next
+    const unsigned rows = a.rows, trips = (rows + p.stride - 1) / p.stride;
+    unsigned row = p.row, ahead = row;  // the row that is fetched next
     auto fetch = [&](int stage) {
-      if (ahead < a.rows) {
+      if (ahead < rows) {
         ring.fetch(stage, 0, gr, l);
         ring.fetch(stage, 2 * U, xr, l);
       }
@@ -496,13 +499,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fetch(i);
     int stage = 0;
-    long long next_pos = a.rot > 0 && row < a.rows ? where.next(a, row) : -1;
-    const int trips = (a.rows + p.stride - 1) / p.stride;
-    for (int t = 0; t < trips; ++t, row += p.stride, dr += step_d) {
-      const bool on = row < a.rows;
+    long long next_pos = a.rot > 0 && row < rows ? where.next(a, row) : -1;
+    for (unsigned t = 0; t < trips; ++t, row += p.stride, dr += step_d) {
+      const bool on = row < rows;
       fetch(stage == 0 ? kStages - 1 : stage - 1);
       const long long pos = on && a.rot > 0 ? checked(a, next_pos) : -1;
-      if (a.rot > 0 && row + p.stride < a.rows) next_pos = where.next(a, row + p.stride);
+      if (a.rot > 0 && row + p.stride < rows) next_pos = where.next(a, row + p.stride);
       float c[U][V], s[U][V];
 #pragma unroll
       for (int u = 0; u < U; ++u)
