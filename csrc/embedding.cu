@@ -362,8 +362,11 @@ __device__ __forceinline__ void emit_row(float* __restrict__ dst, const float (&
     store_f32<V>(dst, o);
     return;
   }
-  // One addition per element and call, so the order of the atomics does not matter; they need no
-  // read of dW here, and flush subnormal sums to zero.
+  // One addition per element and call, so the order of the atomics does not matter, and calls on several
+  // streams may add to one dW.  The global atomic takes a subnormal operand or result (below 2^-126) as
+  // zero: dW is off by less than 2^-125 there.  Keeping such numbers costs more than they are worth: a
+  // load, an addition and a store take 62 us for 32768 x 1024 instead of 44; compare-and-swap for terms
+  // below 2^-101 only, 12 to 15 % more where a tenth of dy is zero (dropout), up to 30 % where half of it is.
   if constexpr (V % 4 == 0) {
 #pragma unroll
     for (int j = 0; j < V; j += 4)
