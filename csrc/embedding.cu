@@ -7,8 +7,9 @@
 // sets kStatusBadShape, gives a row of zeros and adds nothing to dW.
 //
 // Backward.  Adding rows with atomics makes the result depend on the order in which they
-// arrive; here the tokens are sorted by id (stable, so each row's terms come in token order)
-// and every dW row is written once, so equal inputs give equal bits.
+// arrive; here the tokens are sorted by id (stable, so each row's terms lie in token order), a row's
+// terms are added in an order that their positions fix (parts of 8, then across the warps of a chunk,
+// then across chunks) and every dW element is written once: equal inputs give equal bits.
 //
 //  1. embed_sort_kernel: 2^c bins, each of the ids with the same low c bits (frequent tokens, which
 //     vocabularies number low, spread over the bins).  A cluster of four CTAs per bin (two or one where
@@ -24,11 +25,13 @@
 //  3. embed_join_kernel: adds the pieces of each run that crosses chunks, in chunk order.
 //
 // What bounds them, and what they take at 32768 tokens x 1024 columns (B200, 30522 rows, a quarter of
-// the tokens padding): the lookup of fp32 rows into bf16 20 us, DRAM; the sort 10 us, latency (two
-// sweeps of dependent loads, shared-memory counters, a scan); the reduce 29 us when adding (137 MB,
-// 4.7 TB/s) and 41 us when writing every row, DRAM; the join 5.6 us, latency.  In the reduce all rows
-// of a warp (8 tokens x 1 KB) are loaded before the first is added: 20 warps per SM keep 160 KB in
-// flight; 16 tokens per warp left 12 warps and took 38 us, 8 of 32 tokens at a time 46 us.
+// the tokens padding): the lookup of fp32 rows into bf16 20 us, L2 and DRAM (201 MB with the repeated
+// rows); the sort 10 us, latency (two sweeps of dependent loads, shared-memory counters, a scan); the
+// join 5.6 us, latency.  The reduce takes 28 us when adding (101 MB of dy, 29 MB of named rows read and
+// written: 5.6 TB/s; DRAM moves 133 MB, 4.7 TB/s) and 41 us when writing every row (101 MB of dy, 125 MB of
+// dW: 5.5 TB/s): what bounds it is the bytes in flight.  All rows of a warp (8 tokens x 1 KB) are loaded
+// before the first is added: 20 warps per SM keep 160 KB in flight; 16 tokens per warp left 12 warps and
+// took 38 us, 8 of 32 tokens at a time 46 us.
 #include <algorithm>
 #include <atomic>
 

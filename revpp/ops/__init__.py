@@ -126,7 +126,8 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dw: torch.Tensor, scale: 
     outside the table add nothing.  ``accumulate=False`` writes all of ``dw``, with zeros in the rows
     that no token names.  ``accumulate=True`` adds to the rows that tokens name, and takes subnormal
     numbers (below 2^-126) among the old values, the terms and the sums as zero, like other fp32 atomics.
-    The tokens are sorted first and each row is added in token order: equal inputs give equal bits,
+    The tokens are sorted first and each row's terms are added in an order that their positions in the
+    sorted list fix (eight at a time, then across warps and chunks): equal inputs give equal bits,
     unlike the atomics of ``bert_embed_bwd``."""
     V = dw.shape[0]
     if padding_idx is None:
